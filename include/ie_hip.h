@@ -355,6 +355,46 @@ int ie_hip_rmsnorm_qkv_proj(float* q, float* k, float* v, const float* x,
 int ie_hip_rmsnorm_gate_up_silu(float* out, const float* x, const float* norm_weight, float eps,
                                 ie_matrix w_gate, ie_matrix w_up, int T, hipStream_t stream);
 
+/* ------------------------------------------------- 4-bit weight matrices ---
+ * Products over weights of 4 bits with one scale, and optionally one zero
+ * point, per row and group of `group` consecutive columns:
+ *   W[o, k] = (q[o, k] - z[o, k / group]) * s[o, k / group]
+ * No counterpart in the reference, whose weights end at INT8. All members are
+ * device memory:
+ *   data   [rows, cols / 2] bytes: column 2i in the low half of byte i, column
+ *          2i + 1 in the high half; 16-byte aligned
+ *   scale  [rows, ceil(cols / group)] of scale_dtype (IE_KV_F32, _F16 or _BF16)
+ *   zero   [rows, ceil(cols / group)] bytes, or NULL: every zero point is 8
+ * group is 32, 64 or 128; cols a multiple of 32 (the last group may be short). */
+typedef struct ie_matrix_q4 {
+  const void* data;
+  const void* scale;
+  const void* zero;
+  int32_t scale_dtype;
+  int32_t group;
+  int32_t rows, cols;
+} ie_matrix_q4;
+
+/* Bytes of workspace the products below need for T tokens of `cols` columns; 0
+ * (then `workspace` may be NULL) for small T. 16-byte aligned; it needs no
+ * initialisation, and calls that overlap on one workspace race. */
+size_t ie_hip_matmul_q4_workspace_bytes(int T, int cols);
+
+/* ie_hip_matmul, ie_hip_qkv_proj and ie_hip_gate_up_silu over 4-bit matrices,
+ * with the same arguments and a workspace. x must be 16-byte aligned and must
+ * not overlap an output. Each weight is exact; each activation enters with 23
+ * bits, or with 40 below the largest of its token's 128-column block (columns
+ * 128 i .. 128 i + 127), whichever is coarser; sums are f32. A token's result
+ * is the same bit for bit whatever T it is computed in. gate and up share
+ * shape, group and scale type. */
+int ie_hip_matmul_q4(float* y, const float* x, ie_matrix_q4 w, const float* bias, int T,
+                     int accumulate, void* workspace, hipStream_t stream);
+int ie_hip_qkv_proj_q4(float* q, float* k, float* v, const float* x, ie_matrix_q4 w_qkv,
+                       const float* b_qkv, int T, int q_dim, int kv_dim, void* workspace,
+                       hipStream_t stream);
+int ie_hip_gate_up_silu_q4(float* out, const float* x, ie_matrix_q4 w_gate, ie_matrix_q4 w_up, int T,
+                           void* workspace, hipStream_t stream);
+
 /* out[r] = index of the maximum of logits[r, 0..n) for r < R: the greedy
  * token of each row, with the reference CPU argmax's semantics
  * (src/sampler.cpp:26-31): the first strict maximum in index order (ties go
@@ -362,6 +402,77 @@ int ie_hip_rmsnorm_gate_up_silu(float* out, const float* x, const float* norm_we
  * element exceeds -inf. Replaces argmax_rows (src/cuda/kernels.cuh:106,
  * kernels.cu:785-812), which returns INT_MAX for a row of -inf. */
 int ie_hip_argmax_rows(int32_t* out, const float* logits, int R, int n, hipStream_t stream);
+
+/* ------------------------------------------------ from logits to a token ---
+ * What a request may ask of its logits before a token is drawn, per row, all
+ * pointers device memory. The reference does this on the host
+ * (src/sampler.cpp), one row at a time, over logits copied back; biases and
+ * masks are added here. A NULL member asks nothing.
+ *   history       token ids already in the rows' texts; row r's are
+ *                 history[history_start[r] .. + history_len[r]), prompt first.
+ *                 Entries outside [0, history_size) are not read, ids outside
+ *                 [0, n) are skipped; rows may share entries.
+ *   prompt_len    [R] how many of a row's leading entries are its prompt's
+ *                 (NULL: 0). Presence and frequency count the others only.
+ *   repetition    [R] > 0: a token in the history has its logit l divided by it
+ *                 where l > 0, multiplied otherwise (once, however often it occurs)
+ *   presence      [R] subtracted from a token that was generated
+ *   frequency     [R] subtracted once per time that it was
+ *   bias_token,   row r adds bias_value[i] to token bias_token[i] for i in
+ *   bias_value    [bias_start[r], + bias_len[r]) within [0, bias_size); a token
+ *                 listed twice in a row gets the later value
+ *   mask          [mask_rows, ceil(n / 32)] words, bit i % 32 of word i / 32 set
+ *                 where token i is allowed; the others become -inf
+ *   mask_row      [R] the mask row of each row; outside [0, mask_rows): none.
+ *                 NULL: row r has mask row r. */
+typedef struct ie_logit_rules {
+  const int32_t* history;
+  const int32_t* history_start;
+  const int32_t* history_len;
+  const int32_t* prompt_len;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const int32_t* bias_token;
+  const float* bias_value;
+  const int32_t* bias_start;
+  const int32_t* bias_len;
+  const uint32_t* mask;
+  const int32_t* mask_row;
+  int64_t history_size;
+  int64_t bias_size;
+  int32_t mask_rows;
+} ie_logit_rules;
+
+/* out[r, i] = logits[r, i] under the rules, for r < R and i < n:
+ *   l' = in history ? (l > 0 ? l / repetition : l * repetition) : l
+ *   l' = l' - frequency * times - presence * (times > 0)
+ *   l' = l' + bias; -inf where the mask is 0
+ * each step in f32, in this order. out may equal logits; otherwise the two must
+ * not overlap. */
+int ie_hip_adjust_logits(float* out, const float* logits, ie_logit_rules rules, int R, int n,
+                         hipStream_t stream);
+
+/* One token per row, out[r] < n, by inverse CDF at the caller's random number
+ * u[r] in [0, 1) (values outside are brought in, NaN is 0). Replaces the
+ * reference's host sampler (src/sampler.cpp) after its penalty. Row r's tokens
+ * are ordered by logit, ties by index; a prefix of that order is kept:
+ *   top_k[r]  the first k (NULL, <= 0 or >= n: all)
+ *   min_p[r]  those with weight >= min_p * the largest (NULL, <= 0, NaN: all;
+ *             above 1 counts as 1)
+ *   top_p[r]  of what these two leave, the shortest prefix whose weight reaches
+ *             top_p of theirs (NULL, >= 1, NaN: all); <= 0: the first token
+ * with weight exp((l - max l) / temperature[r]); the token is the first in index
+ * order at which the kept weights' running sum passes u * their total. Weights
+ * are whole numbers of 2^-45 of the largest (of 2^-(63 - log2 n) beyond 262,144
+ * tokens) and sums exact, so a row's token does not depend on R or on timing.
+ * temperature <= 0 (or NaN): the largest logit, lowest index on ties. NaN and
+ * -inf logits are never chosen unless a row has nothing else (then 0); +inf ones
+ * share a row among them. All arrays are device memory, [R]. */
+size_t ie_hip_sample_rows_workspace_bytes(int R, int n);
+int ie_hip_sample_rows(int32_t* out, const float* logits, const float* temperature,
+                       const int32_t* top_k, const float* top_p, const float* min_p,
+                       const float* u, int R, int n, void* workspace, hipStream_t stream);
 
 /* ------------------------------------------------------- page allocator ---
  * The page pool / free list / page tables behind BatchRunner (reference:

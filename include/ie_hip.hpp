@@ -187,6 +187,25 @@ inline void rmsnorm_gate_up_silu(float* out, const float* x, const float* norm, 
   check(ie_hip_rmsnorm_gate_up_silu(out, x, norm, eps, wg, wu, T, stream));
 }
 
+/* matmul / qkv_proj / gate_up_silu over 4-bit matrices (no reference
+ * counterpart); workspace of matmul_q4_workspace_bytes(). */
+inline size_t matmul_q4_workspace_bytes(int T, int cols) {
+  return ie_hip_matmul_q4_workspace_bytes(T, cols);
+}
+inline void matmul_q4(float* y, const float* x, const ie_matrix_q4& w, const float* bias, int T,
+                      bool accumulate, void* workspace, hipStream_t stream) {
+  check(ie_hip_matmul_q4(y, x, w, bias, T, accumulate ? 1 : 0, workspace, stream));
+}
+inline void qkv_proj_q4(float* q, float* k, float* v, const float* x, const ie_matrix_q4& w_qkv,
+                        const float* b_qkv, int T, int q_dim, int kv_dim, void* workspace,
+                        hipStream_t stream) {
+  check(ie_hip_qkv_proj_q4(q, k, v, x, w_qkv, b_qkv, T, q_dim, kv_dim, workspace, stream));
+}
+inline void gate_up_silu_q4(float* out, const float* x, const ie_matrix_q4& wg,
+                            const ie_matrix_q4& wu, int T, void* workspace, hipStream_t stream) {
+  check(ie_hip_gate_up_silu_q4(out, x, wg, wu, T, workspace, stream));
+}
+
 /* gather_rows (kernels.cuh:101-102). */
 inline void gather_rows(float* dst, const float* src, const int* rows, int R, int dim,
                         hipStream_t stream) {
@@ -196,6 +215,20 @@ inline void gather_rows(float* dst, const float* src, const int* rows, int R, in
 /* argmax_rows (kernels.cuh:106): the greedy token of each logit row. */
 inline void argmax_rows(int32_t* out, const float* logits, int R, int n, hipStream_t stream) {
   check(ie_hip_argmax_rows(out, logits, R, n, stream));
+}
+
+/* Penalties, biases and masks on logits, and a token per row (see ie_hip.h). */
+inline void adjust_logits(float* out, const float* logits, const ie_logit_rules& rules, int R, int n,
+                          hipStream_t stream) {
+  check(ie_hip_adjust_logits(out, logits, rules, R, n, stream));
+}
+inline size_t sample_rows_workspace_bytes(int R, int n) {
+  return ie_hip_sample_rows_workspace_bytes(R, n);
+}
+inline void sample_rows(int32_t* out, const float* logits, const float* temperature,
+                        const int32_t* top_k, const float* top_p, const float* min_p,
+                        const float* u, int R, int n, void* workspace, hipStream_t stream) {
+  check(ie_hip_sample_rows(out, logits, temperature, top_k, top_p, min_p, u, R, n, workspace, stream));
 }
 
 }  // namespace ie::hip

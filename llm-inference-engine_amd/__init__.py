@@ -53,6 +53,24 @@ class Matrix(ctypes.Structure):
                 ("rows", ctypes.c_int32), ("cols", ctypes.c_int32)]
 
 
+class MatrixQ4(ctypes.Structure):
+    """ie_matrix_q4: 4-bit weights with a scale (and a zero point) per row and group of columns."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("zero", ctypes.c_void_p),
+                ("scale_dtype", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("rows", ctypes.c_int32), ("cols", ctypes.c_int32)]
+
+
+class LogitRules(ctypes.Structure):
+    """ie_logit_rules: what the rows of a step ask of their logits before a token is drawn."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in (
+        "history", "history_start", "history_len", "prompt_len", "repetition", "presence",
+        "frequency", "bias_token", "bias_value", "bias_start", "bias_len", "mask", "mask_row")]
+        + [("history_size", ctypes.c_int64), ("bias_size", ctypes.c_int64),
+           ("mask_rows", ctypes.c_int32)])
+
+
 _vp, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 _SIGS = {
     "ie_hip_last_error": (ctypes.c_char_p, []),
@@ -96,6 +114,13 @@ _SIGS = {
     "ie_hip_qkv_proj": (_i, [_vp, _vp, _vp, _vp, Matrix, _vp, _i, _i, _i, _vp]),
     "ie_hip_rmsnorm_qkv_proj": (_i, [_vp, _vp, _vp, _vp, _vp, _f, Matrix, _vp, _i, _i, _i, _vp]),
     "ie_hip_rmsnorm_gate_up_silu": (_i, [_vp, _vp, _vp, _f, Matrix, Matrix, _i, _vp]),
+    "ie_hip_matmul_q4_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
+    "ie_hip_matmul_q4": (_i, [_vp, _vp, MatrixQ4, _vp, _i, _i, _vp, _vp]),
+    "ie_hip_qkv_proj_q4": (_i, [_vp, _vp, _vp, _vp, MatrixQ4, _vp, _i, _i, _i, _vp, _vp]),
+    "ie_hip_gate_up_silu_q4": (_i, [_vp, _vp, MatrixQ4, MatrixQ4, _i, _vp, _vp]),
+    "ie_hip_adjust_logits": (_i, [_vp, _vp, LogitRules, _i, _i, _vp]),
+    "ie_hip_sample_rows_workspace_bytes": (ctypes.c_size_t, [_i, _i]),
+    "ie_hip_sample_rows": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     "ie_pages_create": (_vp, [_i, _i, _i]),
     "ie_pages_destroy": (None, [_vp]),
     "ie_pages_open_sequence": (_i, [_vp]),
@@ -152,7 +177,7 @@ def _native():
         spec = importlib.util.spec_from_file_location("native_calls", CALLS_PATH)
         calls = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(calls)
-        calls.set_types(torch.float32, torch.float16, torch.bfloat16, Matrix)
+        calls.set_types(torch.float32, torch.float16, torch.bfloat16, Matrix, MatrixQ4, LogitRules)
         _calls = calls
     return _calls
 
@@ -429,6 +454,221 @@ def rmsnorm_gate_up_silu(out, x, norm, eps: float, w_gate: Matrix, w_up: Matrix,
     """gate_up_silu(rmsnorm(x, norm, eps)) in one launch (no reference counterpart)."""
     _check(_native().ie_hip_rmsnorm_gate_up_silu(
         out, x, norm, eps, w_gate, w_up, x.numel() // w_gate.cols, _stream(stream)))
+
+
+# ---------------------------------------- 4-bit weights, logits to tokens ----
+def _tensor(t, name: str, dtype, shape, like=None):
+    """Refuses a tensor the kernels would read wrongly: another type or shape, elements that do
+    not follow each other, another device than `like` (the call's first tensor) or, for that
+    one, than the current device, whose stream the launch goes to."""
+    import torch
+    if t.dtype != dtype:
+        raise IeHipError(EINVAL, f"{name}: expected {dtype}, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise IeHipError(EINVAL, f"{name}: expected shape {tuple(shape)}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise IeHipError(EINVAL, f"{name}: must be contiguous")
+    if like is not None:
+        if t.device != like.device:
+            raise IeHipError(EINVAL, f"{name}: on {t.device}, not on {like.device}")
+    elif not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise IeHipError(EINVAL, f"{name}: on {t.device}, not on the current GPU")
+
+
+def _tokens(x, cols: int, name: str) -> int:
+    """Rows of the activations x [..., cols]; checks x as _tensor does."""
+    import torch
+    _tensor(x, f"{name}: x", torch.float32, None)
+    if x.dim() == 0 or x.shape[-1] != cols:
+        raise IeHipError(EINVAL, f"{name}: x must have {cols} columns")
+    return x.numel() // cols
+
+
+def _rows_of(t, rows: int, cols: int, name: str, like) -> None:
+    """t holds `rows` rows of `cols` f32 values."""
+    import torch
+    _tensor(t, name, torch.float32, None, like)
+    if t.dim() == 0 or t.shape[-1] != cols or t.numel() != rows * cols:
+        raise IeHipError(EINVAL, f"{name}: expected {rows} rows of {cols}, not {tuple(t.shape)}")
+
+
+def _workspace(workspace, need: int, name: str, like):
+    """The workspace checked, or None where the call needs none."""
+    if need == 0:
+        return None
+    if workspace is None:
+        raise IeHipError(EINVAL, f"{name}: needs a workspace of {need} bytes")
+    if workspace.device != like.device:
+        raise IeHipError(EINVAL, f"{name}: workspace on {workspace.device}, not on {like.device}")
+    if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+        raise IeHipError(EINVAL, f"{name}: needs a contiguous workspace of {need} bytes")
+    return workspace
+
+
+def matrix_q4(data, scale, group: int, zero=None) -> MatrixQ4:
+    """An ie_matrix_q4 over device tensors: packed weights, uint8 [rows, cols / 2] (even columns
+    in the low halves); scales [rows, ceil(cols / group)] in float32, float16 or bfloat16; zero
+    points, uint8 of the scales' shape, or None for 8. The tensors are kept with it."""
+    import torch
+    kinds = {torch.float32: KV_F32, torch.float16: KV_F16, torch.bfloat16: KV_BF16}
+    if data.dim() != 2 or data.dtype != torch.uint8 or not data.is_contiguous():
+        raise IeHipError(EINVAL, "matrix_q4: data must be contiguous uint8 [rows, cols / 2]")
+    if group not in (32, 64, 128):
+        raise IeHipError(EINVAL, "matrix_q4: groups must be of 32, 64 or 128 columns")
+    rows, cols = data.shape[0], 2 * data.shape[1]
+    shape = (rows, -(-cols // group))
+    if scale.dtype not in kinds:
+        raise IeHipError(EINVAL, f"matrix_q4: scales of {scale.dtype}")
+    _tensor(scale, "matrix_q4: scale", scale.dtype, shape, data)
+    if zero is not None:
+        _tensor(zero, "matrix_q4: zero", torch.uint8, shape, data)
+    m = MatrixQ4(data.data_ptr(), scale.data_ptr(), None if zero is None else zero.data_ptr(),
+                 kinds[scale.dtype], group, rows, cols)
+    m.tensors = (data, scale, zero)
+    return m
+
+
+def matmul_q4_workspace(T: int, cols: int, device="cuda"):
+    """A workspace for the products of T tokens of `cols` columns (of fewer tokens, too)."""
+    import torch
+    n = int(lib().ie_hip_matmul_q4_workspace_bytes(T, cols))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+
+
+def _q4_workspace(workspace, T: int, w: MatrixQ4, name: str, like):
+    need = int(lib().ie_hip_matmul_q4_workspace_bytes(T, w.cols))
+    return _workspace(workspace, need, name, like)
+
+
+def matmul_q4(y, x, w: MatrixQ4, bias=None, accumulate: bool = False, workspace=None,
+              stream=None) -> None:
+    """matmul() over a 4-bit matrix: y (+)= x . W^T + bias (no reference counterpart)."""
+    T = _tokens(x, w.cols, "matmul_q4")
+    _rows_of(y, T, w.rows, "matmul_q4: y", x)
+    if bias is not None:
+        _rows_of(bias, 1, w.rows, "matmul_q4: bias", x)
+    ws = _q4_workspace(workspace, T, w, "matmul_q4", x)
+    _check(_native().ie_hip_matmul_q4(y, x, w, bias, T, int(accumulate), ws, _stream(stream)))
+
+
+def qkv_proj_q4(q, k, v, x, w_qkv: MatrixQ4, b_qkv=None, workspace=None, stream=None) -> None:
+    """qkv_proj() over a 4-bit matrix (no reference counterpart)."""
+    T = _tokens(x, w_qkv.cols, "qkv_proj_q4")
+    q_dim, kv_dim = q.shape[-1], k.shape[-1]
+    _rows_of(q, T, q_dim, "qkv_proj_q4: q", x)
+    _rows_of(k, T, kv_dim, "qkv_proj_q4: k", x)
+    _rows_of(v, T, kv_dim, "qkv_proj_q4: v", x)
+    if b_qkv is not None:
+        _rows_of(b_qkv, 1, w_qkv.rows, "qkv_proj_q4: bias", x)
+    ws = _q4_workspace(workspace, T, w_qkv, "qkv_proj_q4", x)
+    _check(_native().ie_hip_qkv_proj_q4(q, k, v, x, w_qkv, b_qkv, T, q_dim, kv_dim, ws,
+                                        _stream(stream)))
+
+
+def gate_up_silu_q4(out, x, w_gate: MatrixQ4, w_up: MatrixQ4, workspace=None, stream=None) -> None:
+    """gate_up_silu() over two 4-bit matrices (no reference counterpart)."""
+    T = _tokens(x, w_gate.cols, "gate_up_silu_q4")
+    _rows_of(out, T, w_gate.rows, "gate_up_silu_q4: out", x)
+    ws = _q4_workspace(workspace, T, w_gate, "gate_up_silu_q4", x)
+    _check(_native().ie_hip_gate_up_silu_q4(out, x, w_gate, w_up, T, ws, _stream(stream)))
+
+
+def logit_rules(history=None, prompt_len=None, repetition=None, presence=None, frequency=None,
+                bias=None, mask=None, mask_row=None) -> LogitRules:
+    """The rules of R rows for adjust_logits, over device tensors that are kept with it: history
+    = (token ids, start [R], length [R]) and prompt_len [R], int32; repetition, presence and
+    frequency [R], float32; bias = (tokens int32, values float32, start [R], length [R]); mask
+    [mask rows, ceil(n / 32)] int32 words and mask_row [R] int32 (negative: none)."""
+    import torch
+    i32, f32 = torch.int32, torch.float32
+    r, keep, rows = LogitRules(), [], None
+
+    def put(field, t, dtype, per_row=True):
+        nonlocal rows
+        if per_row:
+            if rows is None:
+                rows = t.numel()
+            _tensor(t, f"logit_rules: {field}", dtype, (rows,), keep[0] if keep else t)
+        else:
+            _tensor(t, f"logit_rules: {field}", dtype, None, keep[0] if keep else t)
+        keep.append(t)
+        setattr(r, field, t.data_ptr())
+
+    if history is not None:
+        put("history", history[0], i32, False)
+        put("history_start", history[1], i32)
+        put("history_len", history[2], i32)
+        r.history_size = history[0].numel()
+    elif any(t is not None for t in (prompt_len, repetition, presence, frequency)):
+        raise IeHipError(EINVAL, "logit_rules: penalties need a history")
+    for field, t, dtype in (("prompt_len", prompt_len, i32), ("repetition", repetition, f32),
+                            ("presence", presence, f32), ("frequency", frequency, f32)):
+        if t is not None:
+            put(field, t, dtype)
+    if bias is not None:
+        put("bias_token", bias[0], i32, False)
+        put("bias_value", bias[1], f32, False)
+        if bias[0].numel() != bias[1].numel():
+            raise IeHipError(EINVAL, "logit_rules: as many bias values as tokens")
+        put("bias_start", bias[2], i32)
+        put("bias_len", bias[3], i32)
+        r.bias_size = bias[0].numel()
+    if mask is not None:
+        put("mask", mask, i32, False)
+        if mask.dim() != 2:
+            raise IeHipError(EINVAL, "logit_rules: mask must be [mask rows, words]")
+        r.mask_rows = mask.shape[0]
+        if mask_row is not None:
+            put("mask_row", mask_row, i32)
+    elif mask_row is not None:
+        raise IeHipError(EINVAL, "logit_rules: mask rows without a mask")
+    r.tensors, r.rows, r.words = tuple(keep), rows, None if mask is None else mask.shape[1]
+    return r
+
+
+def adjust_logits(out, logits, rules: LogitRules, stream=None) -> None:
+    """out = logits [R, n] under the rules (the penalty of src/sampler.cpp, biases and masks);
+    out may be logits."""
+    import torch
+    _tensor(logits, "adjust_logits: logits", torch.float32, None)
+    if logits.dim() != 2:
+        raise IeHipError(EINVAL, "adjust_logits: logits must be [R, n]")
+    R, n = logits.shape
+    _tensor(out, "adjust_logits: out", torch.float32, (R, n), logits)
+    if rules.rows is not None and rules.rows != R:
+        raise IeHipError(EINVAL, f"adjust_logits: rules of {rules.rows} rows for {R}")
+    if rules.words is not None and rules.words != -(-n // 32):
+        raise IeHipError(EINVAL, f"adjust_logits: a mask of {rules.words} words for {n} tokens")
+    if rules.tensors and rules.tensors[0].device != logits.device:
+        raise IeHipError(EINVAL, f"adjust_logits: rules on {rules.tensors[0].device}")
+    _check(_native().ie_hip_adjust_logits(out, logits, rules, R, n, _stream(stream)))
+
+
+def sample_rows_workspace(R: int, n: int, device="cuda"):
+    """A workspace for sample_rows of up to R rows of up to n logits."""
+    import torch
+    b = int(lib().ie_hip_sample_rows_workspace_bytes(R, n))
+    return torch.empty(max(b, 256), dtype=torch.uint8, device=device)
+
+
+def sample_rows(out, logits, temperature, u, top_k=None, top_p=None, min_p=None, workspace=None,
+                stream=None) -> None:
+    """out[r] = a token of logits[r] drawn at u[r] under its temperature, top-k, min-p and top-p
+    (src/sampler.cpp after its penalty); temperature <= 0 takes the largest."""
+    import torch
+    _tensor(logits, "sample_rows: logits", torch.float32, None)
+    if logits.dim() != 2:
+        raise IeHipError(EINVAL, "sample_rows: logits must be [R, n]")
+    R, n = logits.shape
+    for name, t, dtype in (("out", out, torch.int32), ("temperature", temperature, torch.float32),
+                           ("u", u, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None:
+            _tensor(t, f"sample_rows: {name}", dtype, (R,), logits)
+    need = int(lib().ie_hip_sample_rows_workspace_bytes(R, n))
+    ws = _workspace(workspace, need, "sample_rows", logits)
+    _check(_native().ie_hip_sample_rows(out, logits, temperature, top_k, top_p, min_p, u, R, n, ws,
+                                        _stream(stream)))
 
 
 def gather_kv(dst, pool, tables, max_pages: int, seq: int, length: int, kv_dim: int,

@@ -6,8 +6,8 @@
 //
 // Arguments are the C function's, in order: a pointer is None or an object with data_ptr() (a
 // tensor), a stream None or its handle, an integer a Python int; an ie_kv_layout is (tables,
-// max_pages, pool, elements per token row); an ie_matrix the ctypes Matrix. The status code is
-// returned. The GIL is released during the call, as ctypes does.
+// max_pages, pool, elements per token row); an ie_matrix, ie_matrix_q4 or ie_logit_rules the ctypes
+// structure of that name. The status code is returned. The GIL is released during the call, as ctypes does.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -20,9 +20,19 @@
 
 namespace {
 
-// The torch dtypes of IE_KV_F32, IE_KV_F16, IE_KV_BF16, and the Matrix class (set_types).
+// The torch dtypes of IE_KV_F32, IE_KV_F16, IE_KV_BF16, and the classes of the structures passed by
+// value (set_types).
 PyObject* g_dtypes[3] = {nullptr, nullptr, nullptr};
-PyObject* g_matrix = nullptr;
+PyObject* g_structs[3] = {nullptr, nullptr, nullptr};
+template <class T>
+constexpr int kStruct = -1;
+template <>
+constexpr int kStruct<ie_matrix> = 0;
+template <>
+constexpr int kStruct<ie_matrix_q4> = 1;
+template <>
+constexpr int kStruct<ie_logit_rules> = 2;
+constexpr const char* kStructNames[3] = {"Matrix", "MatrixQ4", "LogitRules"};
 PyObject *g_data_ptr = nullptr, *g_numel = nullptr, *g_dtype = nullptr;
 
 bool as_u64(PyObject* o, unsigned long long* v) {
@@ -93,18 +103,18 @@ bool convert(PyObject* o, T* out) {
     if (!as_u64(o, &v)) return false;
     *out = static_cast<T>(v);
     return true;
-  } else if constexpr (std::is_same_v<T, ie_matrix>) {
-    const int is = PyObject_IsInstance(o, g_matrix);
+  } else if constexpr (kStruct<T> >= 0) {
+    const int is = PyObject_IsInstance(o, g_structs[kStruct<T>]);
     if (is <= 0) {
-      if (!is) PyErr_SetString(PyExc_TypeError, "expected a Matrix");
+      if (!is) PyErr_Format(PyExc_TypeError, "expected a %s", kStructNames[kStruct<T>]);
       return false;
     }
     Py_buffer b;
     if (PyObject_GetBuffer(o, &b, PyBUF_SIMPLE)) return false;
-    const bool ok = b.len == Py_ssize_t(sizeof(ie_matrix));
-    if (ok) std::memcpy(out, b.buf, sizeof(ie_matrix));
+    const bool ok = b.len == Py_ssize_t(sizeof(T));
+    if (ok) std::memcpy(out, b.buf, sizeof(T));
     PyBuffer_Release(&b);
-    if (!ok) PyErr_SetString(PyExc_TypeError, "expected a Matrix");
+    if (!ok) PyErr_Format(PyExc_TypeError, "expected a %s", kStructNames[kStruct<T>]);
     return ok;
   } else {
     static_assert(std::is_same_v<T, ie_kv_layout>, "an argument type of ie_hip.h");
@@ -144,12 +154,12 @@ struct Args<R (*)(A...)> {
   static constexpr size_t count = sizeof...(A);
 };
 
-template <bool kMatrices, class T>
+template <bool kStructs, class T>
 bool convert_if(PyObject* o, T* out) {
-  return std::is_same_v<T, ie_matrix> != kMatrices || convert(o, out);
+  return (kStruct<T> >= 0) != kStructs || convert(o, out);
 }
 
-// Matrices first: their check asks no tensor for anything.
+// Structures first: their check asks no tensor for anything.
 template <class T, size_t... I>
 bool convert_all(PyObject* const* args, T& t, std::index_sequence<I...>) {
   return (convert_if<true>(args[I], &std::get<I>(t)) && ...) &&
@@ -173,15 +183,16 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyObject* set_types(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "expected the dtypes of f32, f16 and bf16 and the Matrix class");
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError,
+                    "expected the dtypes of f32, f16 and bf16 and the classes Matrix, MatrixQ4, LogitRules");
     return nullptr;
   }
-  Py_INCREF(args[3]);
-  Py_XSETREF(g_matrix, args[3]);
   for (int i = 0; i < 3; ++i) {
     Py_INCREF(args[i]);
     Py_XSETREF(g_dtypes[i], args[i]);
+    Py_INCREF(args[3 + i]);
+    Py_XSETREF(g_structs[i], args[3 + i]);
   }
   Py_RETURN_NONE;
 }
@@ -209,6 +220,11 @@ PyMethodDef methods[] = {
     IE_CALL(ie_hip_qkv_proj),
     IE_CALL(ie_hip_rmsnorm_qkv_proj),
     IE_CALL(ie_hip_rmsnorm_gate_up_silu),
+    IE_CALL(ie_hip_matmul_q4),
+    IE_CALL(ie_hip_qkv_proj_q4),
+    IE_CALL(ie_hip_gate_up_silu_q4),
+    IE_CALL(ie_hip_adjust_logits),
+    IE_CALL(ie_hip_sample_rows),
     {nullptr, nullptr, 0, nullptr}};
 #undef IE_CALL
 
