@@ -465,10 +465,12 @@ int ie_hip_adjust_logits(float* out, const float* logits, ie_logit_rules rules, 
  * with weight exp((l - max l) / temperature[r]); the token is the first in index
  * order at which the kept weights' running sum passes u * their total. Weights
  * are whole numbers of 2^-45 of the largest (of 2^-(63 - log2 n) beyond 262,144
- * tokens) and sums exact, so a row's token does not depend on R or on timing.
+ * tokens) and their sums exact, so a row's token does not depend on R or on timing.
  * temperature <= 0 (or NaN): the largest logit, lowest index on ties. NaN and
  * -inf logits are never chosen unless a row has nothing else (then 0); +inf ones
- * share a row among them. All arrays are device memory, [R]. */
+ * share a row among them. All arrays are device memory, [R]; n up to 4,194,304.
+ * The workspace (16-byte aligned, sample_rows_workspace_bytes) needs no
+ * initialisation; calls that overlap on one workspace race. */
 size_t ie_hip_sample_rows_workspace_bytes(int R, int n);
 int ie_hip_sample_rows(int32_t* out, const float* logits, const float* temperature,
                        const int32_t* top_k, const float* top_p, const float* min_p,

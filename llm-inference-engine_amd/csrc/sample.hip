@@ -3,12 +3,21 @@
 //
 // A weight is exp((l - max) / T) in float64, taken to whole numbers of 2^-45 (fewer bits where n of
 // them would pass 63: weight_bits): sums of whole numbers are exact, so no order of adding them
-// changes a result, and a border of the sums lies where the 64-bit definition has it to within 2^-46
-// of the largest weight per token.
+// changes a result, and a border of the sums lies where the 64-bit definition has it to within about
+// 2^-45 of the largest weight per token. A row is cut into chunks of kChunk logits, whatever R is.
 //
-// What is kept is a prefix of the tokens ordered by (logit descending, index ascending): its last key
-// is found digit by digit (11 + 11 + 10 bits of the logit's ordered bit pattern) from histograms of
-// counts and weights, its last index among equal logits by counting.
+// What is kept is a prefix of the tokens ordered by (logit descending, index ascending). Four launches,
+// two over (row, chunk) that fill the chip and two over rows:
+//   chunks   the chunk's largest logit, its weight relative to that, and, for rows with a filter, a
+//            histogram of counts and weights over bins of T / 32 in the logit, which every chunk
+//            places alike (place())
+//   border   the row's histogram: which few bins hold the filters' borders; greedy rows end here
+//   collect  per chunk the weight of the bins above all borders; the tokens of the border bins go to
+//            the row's list
+//   draw     the borders, found digit by digit of the ordered bit pattern in that list (of at most
+//            kList tokens; the whole row where the bins hold more, as with a row of equal logits),
+//            then the chunk and the token where the running sum passes the target
+// (64 rows x 151,936, settings mixed: one workgroup a row through all of it took 1,440 us.)
 #include <algorithm>
 #include <cmath>
 
@@ -17,9 +26,14 @@
 namespace iehip {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kEach = 16;                  // logits of a thread
+constexpr int kChunk = kThreads * kEach;
+constexpr int kPlaces = 1024;              // bins of the rows' histograms, a thread each
+constexpr int kList = 4096;                // border tokens of a row
+constexpr int kDigits = 2048;
+constexpr int kMaxTokens = 1 << 22;
+typedef unsigned long long u64;
 
 // Bits of the largest weight, so that n of them stay under 2^63.
 int weight_bits(int n) {
@@ -28,210 +42,714 @@ int weight_bits(int n) {
   return std::min(45, 63 - log2);
 }
 
-// Logits in their order as unsigned numbers; NaN below all, -0 with +0.
+enum Mode { kDone, kAll, kFiltered, kWhole };
+
+// What the border launch leaves of a row. Bins below `sure` are kept whole; those in
+// [outer_lo, outer_hi] hold the border of top-k or min-p, those in [inner_lo, inner_hi] top-p's.
+struct RowState {
+  int32_t mode, listed;
+  float top;
+  int32_t sure, outer_lo, outer_hi, inner_lo, inner_hi;
+  int32_t top_left;      // top-k: how many of the outer bins' tokens stay (INT_MAX: no limit)
+  int32_t pad;
+  u64 sure_mass;         // of the bins below `sure`
+  u64 outer_mass;        // of the bins below outer_lo
+  u64 total;             // of the row
+};
+
+struct Entry {
+  float l;
+  int32_t i;
+};
+
+struct Workspace {
+  RowState* rows;    // [R]
+  Entry* list;       // [R, kList]
+  u64* mass;         // [R, chunks] relative to the chunk's own top; after `collect` its sure weight
+  float* top;        // [R, chunks]
+  int32_t* top_at;   // [R, chunks]
+  u64* bin_mass;     // [R, chunks, kPlaces]
+  uint32_t* bin_count;
+};
+
+size_t lay_out(Workspace* w, void* base, int R, int n) {
+  const size_t chunks = (size_t(n) + kChunk - 1) / kChunk, rc = R * chunks;
+  unsigned char* p = static_cast<unsigned char*>(base);
+  auto take = [&](size_t bytes) {
+    unsigned char* at = p;
+    p += (bytes + 15) / 16 * 16;
+    return at;
+  };
+  Workspace v;
+  v.rows = reinterpret_cast<RowState*>(take(R * sizeof(RowState)));
+  v.list = reinterpret_cast<Entry*>(take(R * size_t(kList) * sizeof(Entry)));
+  v.mass = reinterpret_cast<u64*>(take(rc * 8));
+  v.top = reinterpret_cast<float*>(take(rc * 4));
+  v.top_at = reinterpret_cast<int32_t*>(take(rc * 4));
+  v.bin_mass = reinterpret_cast<u64*>(take(rc * kPlaces * 8));
+  v.bin_count = reinterpret_cast<uint32_t*>(take(rc * kPlaces * 4));
+  if (w) *w = v;
+  return size_t(p - static_cast<unsigned char*>(base));
+}
+
+struct Settings {
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  const float* u;
+};
+
+// One row's settings, brought into their ranges.
+struct Row {
+  double inv, scale, least, one;  // 1 / T, bins per logit, min-p, the largest weight
+  int k;                          // n: no top-k
+  float p;                        // 1: no top-p
+  bool greedy;
+  __device__ __forceinline__ Row(const Settings& s, int row, int n, double one_) : one(one_) {
+    const float t = s.temperature[row];
+    greedy = !(t > 0.0f);
+    inv = 1.0 / double(t);
+    scale = 32.0 * inv;
+    const float m = s.min_p ? s.min_p[row] : 0.0f;
+    least = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
+    k = s.top_k ? s.top_k[row] : 0;
+    if (k <= 0 || k > n) k = n;
+    p = s.top_p ? s.top_p[row] : 1.0f;
+    if (!(p < 1.0f)) p = 1.0f;
+    if (p <= 0.0f) {
+      k = 1;
+      p = 1.0f;
+    }
+    if (k == 1) p = 1.0f;
+  }
+  __device__ __forceinline__ bool filtered(int n) const { return k < n || p < 1.0f || least > 0.0; }
+};
+
+// Logits in their order as unsigned numbers, -0 with +0. (NaN was read as -inf.)
 __device__ __forceinline__ uint32_t order_key(float l) {
-  if (l != l) return 0;
   const uint32_t b = __float_as_uint(l + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-struct Row {
-  float top;     // the largest logit
-  double t;      // temperature
-  double least;  // min-p as a weight
-  double one;    // the largest weight
-};
-
-__device__ __forceinline__ unsigned long long weight(float l, const Row& w) {
-  if (!(l > -INFINITY)) return 0;
-  if (w.top == INFINITY) return l == INFINITY ? static_cast<unsigned long long>(w.one) : 0ull;
-  const double e = exp((double(l) - double(w.top)) / w.t);
-  return e >= w.least ? static_cast<unsigned long long>(__double2ll_rn(e * w.one)) : 0ull;
+// 2^(j / 64) in LDS, for weight_of.
+__device__ __forceinline__ void fill_powers(double* powers) {
+  if (threadIdx.x < 64) powers[threadIdx.x] = exp2(double(threadIdx.x) / 64.0);
 }
 
-struct Bins {
-  uint32_t count[kBins];
-  unsigned long long mass[kBins];
-};
+// exp((l - top) / T) in [0, 1]. With m = round(64 x / ln 2) and r = x - m ln2 / 64, |r| <= 0.0055:
+// 2^(m div 64) 2^(m mod 64 / 64) (1 + r + .. + r^5 / 120), off by less than 2^-50 (r^6 / 720 =
+// 2^-54.5, and the roundings). 17 float64 instructions; the library's exp makes the first launch 64
+// rows x 151,936 half as long again.
+__device__ __forceinline__ double weight_of(float l, float top, double inv, const double* powers) {
+  if (l == top) return 1.0;
+  const double x = (double(l) - double(top)) * inv;
+  if (!(x > -45.0)) return 0.0;  // below 2^-64; l = -inf, top = inf
+  const double m = rint(x * 92.33248261689366);  // 64 / ln 2
+  double r = __builtin_fma(m, -0.010830424696249145, x);
+  r = __builtin_fma(m, -3.623510646634843e-19, r);  // ln2 / 64 less its leading 53 bits
+  double e = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
+  e = __builtin_fma(e, r, 1.0 / 6.0);
+  e = __builtin_fma(e, r, 0.5);
+  e = __builtin_fma(e, r, 1.0);
+  e = __builtin_fma(e, r, 1.0);
+  const int im = int(m);
+  return ldexp(powers[im & 63] * e, im >> 6);
+}
+
+// A weight as a whole number: adding 2^52 leaves it, rounded, in the low bits.
+__device__ __forceinline__ u64 whole(double e, double one) {
+  return static_cast<u64>(__double_as_longlong(__builtin_fma(e, one, 0x1p52))) & 0xFFFFFFFFFFFFFull;
+}
+
+// Where logits stand on the bins' axis: one function of l for every chunk.
+__device__ __forceinline__ double place(float l, double scale) {
+  return l == -INFINITY ? -INFINITY : floor(double(l) * scale);
+}
+__device__ __forceinline__ int bin_below(double top_place, double at) {
+  const double d = top_place - at;
+  return d < double(kPlaces - 1) ? int(d) : (top_place == at ? 0 : kPlaces - 1);
+}
+
+__device__ __forceinline__ float read_logit(float v) { return v == v ? v : -INFINITY; }
+
+// A thread's logits of a chunk: element e of vec4 u is number (u * kThreads + tid) * 4 + e of the chunk.
+__device__ __forceinline__ int chunk_index(int j) {
+  return ((j >> 2) * kThreads + int(threadIdx.x)) * 4 + (j & 3);
+}
+__device__ __forceinline__ void load_chunk(float (&v)[kEach], const float* l, int len, bool vec) {
+#pragma unroll
+  for (int u = 0; u < kEach / 4; ++u) {
+    const int at = chunk_index(4 * u);
+    if (vec && at + 3 < len) {
+      const float4 q = *reinterpret_cast<const float4*>(l + at);
+      v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * u + e] = at + e < len ? l[at + e] : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) v[j] = read_logit(v[j]);
+}
+
+__device__ __forceinline__ u64 wave_sum(u64 m) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m += __shfl_xor(m, off, 64);
+  return m;
+}
+
+__device__ __forceinline__ bool beats(float v, int i, float best, int at) {
+  return v > best || (v == best && i < at);
+}
 
 __global__ void __launch_bounds__(kThreads)
-sample_rows_kernel(int32_t* __restrict__ out, const float* __restrict__ logits,
-                   const float* __restrict__ temperature, const int32_t* __restrict__ top_k,
-                   const float* __restrict__ top_p, const float* __restrict__ min_p,
-                   const float* __restrict__ u, int n, double one) {
-  __shared__ Bins bins;
+sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
+                     double one, int vec) {
+  __shared__ uint32_t count[kPlaces];
+  __shared__ u64 mass[kPlaces];
+  __shared__ double powers[64];
   __shared__ float red_v[kWaves];
   __shared__ int red_i[kWaves];
-  __shared__ unsigned long long red_m[kWaves];
-  __shared__ uint32_t found_bin, found_left;
-  __shared__ unsigned long long found_before;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* l = logits + size_t(row) * n;
-
+  __shared__ u64 red_m[kWaves];
+  __shared__ uint32_t far_count;
+  const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int base = c * kChunk, len = min(kChunk, n - base);
+  float v[kEach];
+  load_chunk(v, logits + size_t(row) * n + base, len, vec);
+  const Row r(s, row, n, one);
+  const bool bins = !r.greedy && r.filtered(n);
+  count[tid] = 0;
+  mass[tid] = 0;
+  if (tid == 0) far_count = 0;
+  fill_powers(powers);
   float best = -INFINITY;
   int at = 0x7fffffff;
-  for (int i = tid; i < n; i += kThreads)
-    if (l[i] > best) {
-      best = l[i];
-      at = i;
-    }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (v[j] > best) best = v[j], at = chunk_index(j);
+#pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
-    const float v = __shfl_xor(best, off, 64);
+    const float o = __shfl_xor(best, off, 64);
     const int i = __shfl_xor(at, off, 64);
-    if (v > best || (v == best && i < at)) best = v, at = i;
+    if (beats(o, i, best, at)) best = o, at = i;
   }
   if (lane == 0) red_v[wave] = best, red_i[wave] = at;
   __syncthreads();
   best = red_v[0], at = red_i[0];
-  for (int w = 1; w < kWaves; ++w)
-    if (red_v[w] > best || (red_v[w] == best && red_i[w] < at)) best = red_v[w], at = red_i[w];
-  if (at == 0x7fffffff) at = 0;
-  const float temp = temperature[row];
-  if (!(temp > 0.0f) || best == -INFINITY) {
-    if (tid == 0) out[row] = at;
+  for (int i = 1; i < kWaves; ++i)
+    if (beats(red_v[i], red_i[i], best, at)) best = red_v[i], at = red_i[i];
+  const size_t rc = size_t(row) * chunks + c;
+  if (tid == 0) {
+    w.top[rc] = best;
+    w.top_at[rc] = best > -INFINITY ? base + at : 0x7fffffff;
+  }
+  if (r.greedy) return;
+  u64 sum = 0;
+  uint32_t far = 0;
+  const double tp = place(best, r.scale);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (chunk_index(j) >= len) continue;
+    const u64 m = v[j] == -INFINITY ? 0 : whole(weight_of(v[j], best, r.inv, powers), one);
+    sum += m;
+    if (!bins) continue;
+    const int b = v[j] == best ? 0 : bin_below(tp, place(v[j], r.scale));
+    if (b == kPlaces - 1) {
+      ++far;  // a masked row's tokens: not one by one
+      if (m) atomicAdd(&mass[b], m);
+    } else {
+      atomicAdd(&count[b], 1u);
+      atomicAdd(&mass[b], m);
+    }
+  }
+  sum = wave_sum(sum);
+  if (lane == 0) red_m[wave] = sum;
+  if (bins) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) far += __shfl_xor(far, off, 64);
+    if (lane == 0 && far) atomicAdd(&far_count, far);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    sum = 0;
+    for (int i = 0; i < kWaves; ++i) sum += red_m[i];
+    w.mass[rc] = sum;
+  }
+  if (!bins) return;
+  w.bin_count[rc * kPlaces + tid] = count[tid] + (tid == kPlaces - 1 ? far_count : 0);
+  w.bin_mass[rc * kPlaces + tid] = mass[tid];
+}
+
+// A chunk's weight, kept relative to its own largest logit, on the row's scale.
+__device__ __forceinline__ u64 rescale(u64 m, float chunk_top, float top, double inv, const double* powers) {
+  if (!m || chunk_top == top) return m;
+  return static_cast<u64>(rint(double(m) * weight_of(chunk_top, top, inv, powers)));
+}
+
+// Running sums over the workgroup's threads, own value included.
+struct Scan {
+  u64 mass[kWaves];
+  uint32_t count[kWaves];
+};
+__device__ __forceinline__ void scan(Scan& sh, u64& m, uint32_t& c) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const u64 om = __shfl_up(m, off, 64);
+    const uint32_t oc = __shfl_up(c, off, 64);
+    if (lane >= off) m += om, c += oc;
+  }
+  __syncthreads();
+  if (lane == 63) sh.mass[wave] = m, sh.count[wave] = c;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) m += sh.mass[i], c += sh.count[i];
+}
+
+__global__ void __launch_bounds__(kThreads)
+sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, int chunks, double one) {
+  __shared__ uint32_t count[kPlaces];
+  __shared__ u64 mass[kPlaces];
+  __shared__ double powers[64];
+  __shared__ Scan sh;
+  __shared__ float red_v[kWaves];
+  __shared__ int red_i[kWaves];
+  __shared__ int found[3];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Row r(s, row, n, one);
+  const float* tops = w.top + size_t(row) * chunks;
+  count[tid] = 0;
+  mass[tid] = 0;
+  if (tid < 3) found[tid] = kPlaces - 1;
+  fill_powers(powers);
+  float top = -INFINITY;
+  int at = 0x7fffffff;
+  for (int c = tid; c < chunks; c += kThreads) {
+    const int i = w.top_at[size_t(row) * chunks + c];
+    if (beats(tops[c], i, top, at)) top = tops[c], at = i;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const float o = __shfl_xor(top, off, 64);
+    const int i = __shfl_xor(at, off, 64);
+    if (beats(o, i, top, at)) top = o, at = i;
+  }
+  if (lane == 0) red_v[wave] = top, red_i[wave] = at;
+  __syncthreads();
+  top = red_v[0], at = red_i[0];
+  for (int i = 1; i < kWaves; ++i)
+    if (beats(red_v[i], red_i[i], top, at)) top = red_v[i], at = red_i[i];
+  RowState* st = w.rows + row;
+  if (r.greedy || at == 0x7fffffff || !r.filtered(n)) {
+    if (tid == 0) {
+      st->mode = r.greedy || at == 0x7fffffff ? kDone : kAll;
+      st->top = top;
+      if (st->mode == kDone) out[row] = at == 0x7fffffff ? 0 : at;
+    }
     return;
   }
-  Row w;
-  w.top = best;
-  w.t = temp;
-  w.one = one;
-  const float mp = min_p ? min_p[row] : 0.0f;
-  w.least = mp > 0.0f ? fmin(double(mp), 1.0) : 0.0;
-  int k = top_k ? top_k[row] : 0;
-  if (k <= 0 || k > n) k = n;
-  const float tp = top_p ? top_p[row] : 1.0f;
-  const bool by_mass = tp < 1.0f;
-  if (by_mass && tp <= 0.0f) k = 1;
+  const double tp = place(top, r.scale);
+  for (int c = 0; c < chunks; ++c) {
+    const size_t rc = size_t(row) * chunks + c;
+    const uint32_t cc = w.bin_count[rc * kPlaces + tid];
+    if (!cc) continue;
+    const int d = tops[c] == top ? 0 : bin_below(tp, place(tops[c], r.scale));
+    const int b = min(tid + d, kPlaces - 1);
+    atomicAdd(&count[b], cc);
+    const u64 m = rescale(w.bin_mass[rc * kPlaces + tid], tops[c], top, r.inv, powers);
+    if (m) atomicAdd(&mass[b], m);
+  }
+  __syncthreads();
+  u64 cm = mass[tid];
+  uint32_t cn = count[tid];
+  const uint32_t own_n = cn;
+  const u64 own_m = cm;
+  scan(sh, cm, cn);
+  __syncthreads();
+  count[tid] = cn;  // running sums from here on
+  mass[tid] = cm;
+  const u64 bm = cm - own_m;
+  const uint32_t bn = cn - own_n;
+  // top-k's bin: the one in which the running count reaches k
+  if (bn < uint32_t(r.k) && cn >= uint32_t(r.k)) found[0] = tid;
+  __syncthreads();
+  const bool by_count = r.k < n;
+  int lo = 0x7fffffff, hi = -1, left = 0x7fffffff;
+  if (r.least > 0.0) {
+    // min-p's: one bin to either side of where its logit falls, for the roundings of the two
+    const double at_least = top == INFINITY ? 0.0 : (double(top) + log(r.least) / r.inv) * r.scale;
+    const double d = top == INFINITY ? 0.0 : tp - floor(at_least);
+    const int b = d < double(kPlaces - 1) ? int(fmax(d, 0.0)) : kPlaces - 1;
+    lo = max(b - 1, 0);
+    hi = min(b + 1, kPlaces - 1);
+  }
+  if (by_count) {
+    const int b = found[0];
+    if (b < lo) {
+      lo = hi = b;
+    } else {
+      hi = min(hi, b);
+    }
+    if (b <= hi) left = r.k - (lo ? int(count[lo - 1]) : 0);
+  }
+  const bool outer = hi >= 0;
+  const u64 total = mass[kPlaces - 1];
+  const u64 below = outer ? (lo ? mass[lo - 1] : 0) : total;
+  const u64 above = outer ? mass[hi] : total;
+  if (r.p < 1.0f) {
+    const double glo = double(r.p) * double(below), ghi = double(r.p) * double(above);
+    if ((tid == 0 || double(bm) < glo) && double(cm) >= glo) found[1] = tid;
+    if ((tid == 0 || double(bm) < ghi) && double(cm) >= ghi) found[2] = tid;
+  }
+  __syncthreads();
+  if (tid != 0) return;
+  RowState o;
+  o.top = top;
+  o.outer_lo = outer ? lo : kPlaces;
+  o.outer_hi = outer ? hi : kPlaces;
+  o.inner_lo = r.p < 1.0f ? found[1] : kPlaces;
+  o.inner_hi = r.p < 1.0f ? (outer ? min(found[2], hi) : found[2]) : kPlaces;
+  if (o.inner_lo > o.inner_hi) o.inner_lo = o.inner_hi;
+  o.sure = min(o.outer_lo, o.inner_lo);
+  o.sure_mass = o.sure ? mass[o.sure - 1] : 0;
+  o.outer_mass = below;
+  o.total = total;
+  o.top_left = left;
+  o.pad = 0;
+  o.listed = 0;
+  auto between = [&](int a, int b) { return a >= kPlaces ? 0u : count[b] - (a ? count[a - 1] : 0u); };
+  uint32_t many = between(o.outer_lo, o.outer_hi);
+  if (o.inner_lo < kPlaces) {
+    if (o.outer_lo >= kPlaces || o.inner_hi < o.outer_lo)
+      many += between(o.inner_lo, o.inner_hi);
+    else if (o.inner_lo < o.outer_lo)
+      many = between(o.inner_lo, o.outer_hi);
+  }
+  o.mode = many <= uint32_t(kList) ? kFiltered : kWhole;
+  *st = o;
+}
 
-  // The kept prefix so far: keys above `key`, and those equal to it up to index `last`.
+__global__ void __launch_bounds__(kThreads)
+sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
+                      double one, int vec) {
+  __shared__ double powers[64];
+  __shared__ u64 red_m[kWaves];
+  __shared__ int many, next;
+  const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
+  RowState* st = w.rows + row;
+  if (st->mode != kFiltered) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const size_t rc = size_t(row) * chunks + c;
+  const int sure = st->sure, outer_lo = st->outer_lo, outer_hi = st->outer_hi;
+  const int inner_lo = st->inner_lo, inner_hi = st->inner_hi;
+  const float top = st->top, chunk_top = w.top[rc];
+  const Row r(s, row, n, one);
+  const double tp = place(top, r.scale);
+  const int nearest = chunk_top == top ? 0 : bin_below(tp, place(chunk_top, r.scale));
+  const int last = max(sure - 1, max(outer_hi < kPlaces ? outer_hi : -1, inner_hi < kPlaces ? inner_hi : -1));
+  if (nearest > last) {
+    if (tid == 0) w.mass[rc] = 0;
+    return;
+  }
+  const int base = c * kChunk, len = min(kChunk, n - base);
+  float v[kEach];
+  load_chunk(v, logits + size_t(row) * n + base, len, vec);
+  fill_powers(powers);
+  if (tid == 0) many = 0;
+  __syncthreads();
+  u64 sum = 0;
+  uint32_t listed = 0;  // a bit per logit
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (chunk_index(j) >= len) continue;
+    const int b = v[j] == top ? 0 : bin_below(tp, place(v[j], r.scale));
+    if (b < sure)
+      sum += whole(weight_of(v[j], top, r.inv, powers), one);
+    else if ((b >= outer_lo && b <= outer_hi) || (b >= inner_lo && b <= inner_hi))
+      listed |= 1u << j;
+  }
+  sum = wave_sum(sum);
+  if (lane == 0) red_m[wave] = sum;
+  int at = listed ? atomicAdd(&many, __popc(listed)) : 0;
+  __syncthreads();
+  if (tid == 0) {
+    sum = 0;
+    for (int i = 0; i < kWaves; ++i) sum += red_m[i];
+    w.mass[rc] = sum;
+    next = many ? atomicAdd(&st->listed, many) : 0;
+  }
+  __syncthreads();
+  at += next;
+  Entry* list = w.list + size_t(row) * kList;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (listed >> j & 1) {
+      if (at < kList) list[at] = Entry{v[j], base + chunk_index(j)};
+      ++at;
+    }
+}
+
+struct Digits {
+  u64 mass[kDigits];
+  uint32_t count[kDigits];
+  Scan scan;
+  int bin;
+  uint32_t before_count, in_count;
+  u64 before_mass;
+};
+
+// One digit over `items` tokens: digit(i, mass) gives a token's bin (-1: none) and weight; the bin
+// in which reach(running count, running mass) first holds is left in d (d.bin = -1: in none).
+template <class Digit, class Reach>
+__device__ __forceinline__ void digit_pass(Digits& d, int items, const Digit& digit, const Reach& reach) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < kDigits; i += kThreads) d.mass[i] = 0, d.count[i] = 0;
+  if (tid == 0) d.bin = -1;
+  __syncthreads();
+  for (int i0 = 0; i0 < items; i0 += kThreads) {
+    u64 m = 0;
+    const int i = i0 + tid, b = i < items ? digit(i, m) : -1;
+    // Equal logits fall into one bin: a wave's as one.
+    const int first = __builtin_amdgcn_readfirstlane(b);
+    if (__all(b == first)) {
+      if (first < 0) continue;
+      m = wave_sum(m);
+      if ((tid & 63) == 0) {
+        atomicAdd(&d.count[first], 64u);
+        if (m) atomicAdd(&d.mass[first], m);
+      }
+    } else if (b >= 0) {
+      atomicAdd(&d.count[b], 1u);
+      if (m) atomicAdd(&d.mass[b], m);
+    }
+  }
+  __syncthreads();
+  const uint32_t n0 = d.count[2 * tid], n1 = d.count[2 * tid + 1];
+  const u64 m0 = d.mass[2 * tid], m1 = d.mass[2 * tid + 1];
+  u64 cm = m0 + m1;
+  uint32_t cn = n0 + n1;
+  scan(d.scan, cm, cn);
+  const u64 bm = cm - m0 - m1;
+  const uint32_t bn = cn - n0 - n1;
+  const bool r0 = reach(bn, bm), r1 = reach(bn + n0, bm + m0), r2 = reach(cn, cm);
+  if (!r0 && r1) d.bin = 2 * tid, d.before_count = bn, d.before_mass = bm, d.in_count = n0;
+  if (!r1 && r2) d.bin = 2 * tid + 1, d.before_count = bn + n0, d.before_mass = bm + m0, d.in_count = n1;
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kThreads)
+sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, Settings s, Workspace w,
+                   int n, int chunks, double one) {
+  __shared__ Digits d;
+  __shared__ Entry list[kList];
+  __shared__ double powers[64];
+  __shared__ u64 chunk_mass[kMaxTokens / kChunk];
+  __shared__ u64 red_m[kWaves];
+  __shared__ u64 before_of;
+  __shared__ int chosen;
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  RowState st = w.rows[row];
+  if (st.mode == kDone) return;
+  const float* l = logits + size_t(row) * n;
+  const Row r(s, row, n, one);
+  const bool filtered = st.mode != kAll, all = st.mode == kWhole;
+  const double tp = place(st.top, r.scale);
+  fill_powers(powers);
+  if (all) {
+    st.sure = 0, st.outer_lo = 0, st.outer_hi = kPlaces - 1, st.inner_lo = 0, st.inner_hi = kPlaces - 1;
+    st.sure_mass = st.outer_mass = 0;
+    st.top_left = r.k < n ? r.k : 0x7fffffff;
+  }
+  const int items = !filtered ? 0 : all ? n : min(st.listed, kList);
+  if (filtered && !all)
+    for (int i = tid; i < items; i += kThreads) list[i] = w.list[size_t(row) * kList + i];
+  for (int i = tid; i < chunks; i += kThreads) {
+    const size_t rc = size_t(row) * chunks + i;
+    chunk_mass[i] = filtered && !all ? w.mass[rc] : 0;
+  }
+  __syncthreads();
+  auto entry = [&](int i) { return all ? Entry{read_logit(l[i]), i} : list[i]; };
+  auto bin_of = [&](float v) { return v == st.top ? 0 : bin_below(tp, place(v, r.scale)); };
+  auto weight = [&](float v) { return weight_of(v, st.top, r.inv, powers); };
+
+  // The kept part of the list: at or above (key, last index), in order, of bins up to `end`, with the
+  // least weight where the bin is one of the outer ones.
   uint32_t key = 0;
-  int last = n - 1;
-  auto kept = [&](float v, int i) {
+  int last = 0x7fffffff, end = kPlaces - 1;
+  auto above = [&](float v, int i) {
     const uint32_t o = order_key(v);
     return o > key || (o == key && i <= last);
   };
-  for (int pass = 0; pass < 2; ++pass) {  // by count, then by weight
-    if (pass == 0 ? k >= n : !by_mass || tp <= 0.0f) continue;
-    double goal = 0;
-    if (pass == 1) {
-      unsigned long long m = 0;
-      for (int i = tid; i < n; i += kThreads)
-        if (kept(l[i], i)) m += weight(l[i], w);
-      for (int off = 32; off > 0; off >>= 1) m += __shfl_xor(m, off, 64);
-      __syncthreads();
-      if (lane == 0) red_m[wave] = m;
-      __syncthreads();
-      m = 0;
-      for (int i = 0; i < kWaves; ++i) m += red_m[i];
-      goal = double(tp) * double(m);
-    }
-    uint32_t prefix = 0, left = k;  // left: how many of the current digit's tokens stay
-    unsigned long long before = 0;  // what stands above the current digit
-    uint32_t count_before = 0;
-    for (int d = 0; d < 3; ++d) {
-      const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kThreads) bins.count[i] = 0, bins.mass[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kThreads) {
-        const uint32_t o = order_key(l[i]);
-        if (d > 0 && (o >> (shift + bits)) != prefix) continue;
-        if (!kept(l[i], i)) continue;
-        const uint32_t b = (o >> shift) & ((1u << bits) - 1);
-        atomicAdd(&bins.count[b], 1u);
-        if (pass == 1) atomicAdd(&bins.mass[b], weight(l[i], w));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        for (int b = (1 << bits) - 1; b >= 0; --b) {
-          if (!bins.count[b]) continue;
-          const bool here = pass == 0 ? count_before + bins.count[b] >= uint32_t(k)
-                                      : double(before + bins.mass[b]) >= goal;
-          if (here) {
-            found_bin = b;
-            found_before = before;
-            found_left = count_before;
-            break;
-          }
-          before += bins.mass[b];
-          count_before += bins.count[b];
-        }
-      }
-      __syncthreads();
-      prefix = (prefix << bits) | found_bin;
-      before = found_before;
-      count_before = found_left;
-      left = bins.count[found_bin];
-      __syncthreads();
-    }
-    // `left` tokens share the last key: how many of them stay, and the index of the last.
-    uint32_t stay;
-    if (pass == 0) {
-      stay = k - count_before;
-    } else {
-      const unsigned long long one = bins.mass[found_bin] / left;
-      const double need = (goal - double(before)) / double(one);
-      stay = need <= 1.0 ? 1u : uint32_t(fmin(ceil(need), double(left)));
-    }
-    const int old_last = prefix == key ? last : n - 1;
-    if (wave == 0) {
-      uint32_t seen = 0;
-      int end = n - 1;
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        const int i = i0 + lane;
-        const bool eq = i < n && i <= old_last && order_key(l[i]) == prefix;
-        const unsigned long long b = __ballot(eq);
-        const uint32_t here = __popcll(b);
-        if (seen + here >= stay) {
-          const uint32_t rank = seen + __popcll(b & ((1ull << lane) - 1)) + 1;
-          const unsigned long long hit = __ballot(eq && rank == stay);
-          end = i0 + __ffsll(hit) - 1;
-          break;
-        }
-        seen += here;
-      }
-      if (lane == 0) found_bin = uint32_t(end);
-    }
-    __syncthreads();
-    key = prefix;
-    last = int(found_bin);
-    __syncthreads();
-  }
-
-  // The draw: each wave's stretch of the row, then the one the target falls in.
-  const int per = (n + kWaves * 64 - 1) / (kWaves * 64) * 64;
-  const int lo = min(n, wave * per), hi = min(n, lo + per);
-  auto part = [&](int i) {
-    return i < hi && kept(l[i], i) ? weight(l[i], w) : 0ull;
+  auto outer = [&](int b) { return b >= st.outer_lo && b <= st.outer_hi; };
+  auto stays = [&](float v, int i, int b, double e) {
+    return b <= end && above(v, i) && (!outer(b) || e >= r.least);
   };
-  unsigned long long m = 0;
-  for (int i = lo + lane; i < hi; i += 64) m += part(i);
-  for (int off = 32; off > 0; off >>= 1) m += __shfl_xor(m, off, 64);
+  // Moves (key, last) to the token at which reach() first holds of the running sums over the tokens
+  // that `take` lets in; `stay` says how many of the last key's equal tokens that is.
+  auto select = [&](const auto& take, const auto& reach, const auto& stay) {
+    uint32_t prefix = 0, n0 = 0;
+    u64 m0 = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      digit_pass(
+          d, items,
+          [&](int i, u64& m) {
+            const Entry e = entry(i);
+            const uint32_t o = order_key(e.l);
+            if (pass > 0 && (o >> (shift + bits)) != prefix) return -1;
+            return take(e.l, e.i, m) ? int(((1u << bits) - 1) - ((o >> shift) & ((1u << bits) - 1))) : -1;
+          },
+          [&](uint32_t c, u64 m) { return reach(n0 + c, m0 + m); });
+      if (d.bin < 0) return;  // never: all stay
+      prefix = (prefix << bits) | (((1u << bits) - 1) - uint32_t(d.bin));
+      n0 += d.before_count;
+      m0 += d.before_mass;
+    }
+    const uint32_t equal = d.in_count, keep = equal > 1 ? stay(equal, n0, m0, prefix) : 1;
+    int to = 0x7fffffff;
+    if (keep < equal) {  // the index of the keep-th of them
+      int high = 0;
+      uint32_t c0 = 0;
+      for (int pass = 0; pass < 2; ++pass) {
+        digit_pass(
+            d, items,
+            [&](int i, u64& m) {
+              const Entry e = entry(i);
+              if (order_key(e.l) != prefix || (pass == 1 && e.i >> 11 != high)) return -1;
+              const int at = pass == 0 ? e.i >> 11 : e.i & 2047;
+              const bool in = take(e.l, e.i, m);
+              m = 0;
+              return in ? at : -1;
+            },
+            [&](uint32_t c, u64) { return c0 + c >= keep; });
+        if (pass == 0) high = d.bin, c0 = d.before_count;
+      }
+      to = (high << 11) | d.bin;
+    }
+    key = prefix;
+    last = to;
+  };
+
+  if (filtered && st.top_left != 0x7fffffff) {
+    const uint32_t left = uint32_t(st.top_left);
+    select([&](float v, int, u64&) { return outer(bin_of(v)); },
+           [&](uint32_t c, u64) { return c >= left; },
+           [&](uint32_t, uint32_t c, u64, uint32_t) { return left - c; });
+  }
+  if (filtered && r.p < 1.0f) {
+    u64 m = 0;
+    for (int i = tid; i < items; i += kThreads) {
+      const Entry e = entry(i);
+      const int b = bin_of(e.l);
+      const double x = weight(e.l);
+      if (outer(b) && stays(e.l, e.i, b, x)) m += whole(x, one);
+    }
+    m = wave_sum(m);
+    __syncthreads();
+    if (lane == 0) red_m[wave] = m;
+    __syncthreads();
+    u64 of = st.outer_lo < kPlaces ? st.outer_mass : st.total;
+    for (int i = 0; i < kWaves; ++i) of += red_m[i];
+    const double goal = double(r.p) * double(of);
+    end = st.inner_hi;
+    select(
+        [&](float v, int i, u64& m) {
+          const int b = bin_of(v);
+          const double x = weight(v);
+          m = whole(x, one);
+          return stays(v, i, b, x);
+        },
+        [&](uint32_t, u64 m) { return double(st.sure_mass + m) >= goal; },
+        [&](uint32_t equal, uint32_t, u64 m, uint32_t o) {
+          const float v = __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+          const double each = double(whole(weight(v), one));
+          const double need = (goal - double(st.sure_mass + m)) / each;
+          return need <= 1.0 ? 1u : uint32_t(fmin(ceil(need), double(equal)));
+        });
+  }
+  // The kept weight of each chunk.
+  if (!filtered) {
+    for (int i = tid; i < chunks; i += kThreads) {
+      const size_t rc = size_t(row) * chunks + i;
+      chunk_mass[i] = rescale(w.mass[rc], w.top[rc], st.top, r.inv, powers);
+    }
+  }
+  auto kept = [&](float v, int i) -> u64 {
+    if (!(v > -INFINITY)) return 0;
+    const double x = weight(v);
+    if (filtered) {
+      const int b = bin_of(v);
+      const bool listed = outer(b) || (b >= st.inner_lo && b <= st.inner_hi);
+      if (b >= st.sure && !(listed && stays(v, i, b, x))) return 0;
+    }
+    return whole(x, one);
+  };
+  __syncthreads();
+  for (int i0 = 0; i0 < items; i0 += kThreads) {
+    const int i = i0 + tid;
+    const Entry e = i < items ? entry(i) : Entry{-INFINITY, 0};
+    u64 m = kept(e.l, e.i);
+    if (all) {  // a wave's tokens are of one chunk
+      m = wave_sum(m);
+      if (lane == 0 && m) atomicAdd(&chunk_mass[e.i / kChunk], m);
+    } else if (m) {
+      atomicAdd(&chunk_mass[e.i / kChunk], m);
+    }
+  }
+  __syncthreads();
+  u64 cm = tid < chunks ? chunk_mass[tid] : 0;
+  const u64 own = cm;
+  uint32_t unused = 0;
+  scan(d.scan, cm, unused);
+  if (tid == kThreads - 1) before_of = cm;
+  __syncthreads();
+  const u64 total = before_of;
+  float u = s.u[row];
+  u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
+  // The first running sum above u * total, in whole numbers: the first that reaches `need`.
+  const u64 need = min(static_cast<u64>(double(u) * double(total)) + 1, total);
+  __syncthreads();
+  if (cm - own < need && cm >= need) chosen = tid, before_of = cm - own;
+  __syncthreads();
+  const int base = chosen * kChunk, len = min(kChunk, n - base);
+  u64 want = need - before_of;
+  if (!filtered) {  // in the chunk's own units, whose sum is at hand
+    const size_t rc = size_t(row) * chunks + chosen;
+    const float chunk_top = w.top[rc];
+    if (chunk_top != st.top) {
+      const double f = weight(chunk_top);
+      want = max(u64(1), min(w.mass[rc], static_cast<u64>(ceil(double(want) / f))));
+      st.top = chunk_top;
+    }
+  }
+  constexpr int kPart = kChunk / kWaves;
+  const int lo = min(len, wave * kPart), hi = min(len, lo + kPart);
+  u64 m = 0;
+  for (int i = lo + lane; i < hi; i += 64) m += kept(read_logit(l[base + i]), base + i);
+  m = wave_sum(m);
   __syncthreads();
   if (lane == 0) red_m[wave] = m;
   __syncthreads();
-  unsigned long long total = 0, mine = 0;
-  for (int i = 0; i < kWaves; ++i) {
-    if (i == wave) mine = total;
-    total += red_m[i];
-  }
-  float r = u[row];
-  r = r > 0.0f ? fminf(r, 0x1.fffffep-1f) : 0.0f;
-  const double target = double(r) * double(total);
-  if (!(double(mine) <= target && target < double(mine + m))) return;
-  unsigned long long sum = mine;
+  u64 mine = 0;
+  for (int i = 0; i < wave; ++i) mine += red_m[i];
+  if (!(mine < want && mine + m >= want)) return;
+  u64 sum = mine;
   for (int i0 = lo; i0 < hi; i0 += 64) {
-    const unsigned long long p = part(i0 + lane);
-    unsigned long long s = p;
+    const int i = i0 + lane;
+    u64 p = i < hi ? kept(read_logit(l[base + i]), base + i) : 0;
+#pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const unsigned long long o = __shfl_up(s, off, 64);
-      if (lane >= off) s += o;
+      const u64 o = __shfl_up(p, off, 64);
+      if (lane >= off) p += o;
     }
-    const unsigned long long past = __ballot(double(sum + s) > target);
+    const u64 past = __ballot(sum + p >= want);
     if (past) {
-      if (lane == 0) out[row] = i0 + __ffsll(past) - 1;
+      if (lane == 0) out[row] = base + i0 + __ffsll(past) - 1;
       return;
     }
-    sum += __shfl(s, 63, 64);
+    sum += __shfl(p, 63, 64);
   }
 }
 
@@ -241,20 +759,33 @@ sample_rows_kernel(int32_t* __restrict__ out, const float* __restrict__ logits,
 using namespace iehip;
 
 extern "C" size_t ie_hip_sample_rows_workspace_bytes(int R, int n) {
-  (void)R;
-  (void)n;
-  return 0;
+  if (R <= 0 || n <= 0 || n > kMaxTokens) return 0;
+  return lay_out(nullptr, nullptr, R, n);
 }
 
 extern "C" int ie_hip_sample_rows(int32_t* out, const float* logits, const float* temperature,
                                   const int32_t* top_k, const float* top_p, const float* min_p,
                                   const float* u, int R, int n, void* workspace, hipStream_t stream) {
   clear_error();
-  (void)workspace;
-  if (R < 0 || n <= 0 || n > (1 << 30)) return fail(IE_HIP_EINVAL, "sample_rows: bad sizes");
+  if (R < 0 || n <= 0) return fail(IE_HIP_EINVAL, "sample_rows: bad sizes");
+  if (n > kMaxTokens) return fail(IE_HIP_EINVAL, "sample_rows: more than 4,194,304 tokens");
   if (R == 0) return IE_HIP_OK;
   if (!out || !logits || !temperature || !u) return fail(IE_HIP_EINVAL, "sample_rows: null pointer");
-  hipLaunchKernelGGL(sample_rows_kernel, dim3(R), dim3(kThreads), 0, stream, out, logits, temperature,
-                     top_k, top_p, min_p, u, n, std::ldexp(1.0, weight_bits(n)));
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(IE_HIP_EINVAL, "sample_rows: needs a 16-byte aligned workspace");
+  const int chunks = (n + kChunk - 1) / kChunk;
+  if (int64_t(R) * chunks * kThreads > int64_t(UINT32_MAX))
+    return fail(IE_HIP_EINVAL, "sample_rows: too many rows");
+  Workspace w;
+  lay_out(&w, workspace, R, n);
+  const Settings s{temperature, top_k, top_p, min_p, u};
+  const double one = std::ldexp(1.0, weight_bits(n));
+  const int vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && n % 4 == 0;
+  const dim3 every(unsigned(R) * chunks), rows(R), block(kThreads);
+  hipLaunchKernelGGL(sample_chunks_kernel, every, block, 0, stream, logits, s, w, n, chunks, one, vec);
+  hipLaunchKernelGGL(sample_border_kernel, rows, block, 0, stream, out, s, w, n, chunks, one);
+  if (top_k || top_p || min_p)
+    hipLaunchKernelGGL(sample_collect_kernel, every, block, 0, stream, logits, s, w, n, chunks, one, vec);
+  hipLaunchKernelGGL(sample_draw_kernel, rows, block, 0, stream, out, logits, s, w, n, chunks, one);
   return check_launch("sample_rows");
 }
