@@ -278,6 +278,310 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
   }
 }
 
+// ---- many tokens: the activations are split once, by a launch of their own ----
+//
+// The workspace holds, per tile of 16 tokens and block of 128 columns, 8 KB of parts as the products
+// take them (hi, then lo: 4 steps x 64 lanes x 16 bytes), then per tile and block the 16 powers of two.
+struct Parts {
+  unsigned char* parts;
+  float* back;
+};
+constexpr int kPartBytes = 8192;
+__host__ __device__ inline size_t part_tiles(int T) { return (size_t(T) + 15) / 16; }
+
+template <bool WIDE>
+__global__ void __launch_bounds__(256)
+q4_split_kernel(Parts out, const float* __restrict__ x, int T, int cols, int blocks) {
+  // 16 lanes per (token, block), so a workgroup is one tile and block.
+  const size_t tile = blockIdx.x / blocks, b = blockIdx.x - tile * blocks;
+  const int t = threadIdx.x >> 4, k8 = threadIdx.x & 15, k = int(b) * kBlock + 8 * k8;
+  const size_t tok = tile * 16 + t;
+  float v[8] = {};
+  if (tok < size_t(T) && k < cols) {
+    const float4* src = reinterpret_cast<const float4*>(x + tok * cols + k);
+    const float4 v0 = src[0], v1 = src[1];
+    v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w;
+    v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
+  }
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) largest = max(largest, finite_bits(v[i]));
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) largest = max(largest, uint32_t(__shfl_xor(int(largest), off, 64)));
+  float factor, back;
+  block_scale(largest, factor, back);
+  f16x8 hi, lo;
+  split8(v, factor, hi, lo);
+  const int step = WIDE ? k8 & 3 : k8 >> 2, g = WIDE ? k8 >> 2 : k8 & 3;
+  unsigned char* to = out.parts + (tile * blocks + b) * kPartBytes + (step * 64 + 16 * g + t) * 16;
+  *reinterpret_cast<f16x8*>(to) = hi;
+  *reinterpret_cast<f16x8*>(to + 4096) = lo;
+  if (k8 == 0) out.back[(tile * blocks + b) * 16 + t] = back;
+}
+
+// A lane's weights, scales and zero points of one block.
+template <int RT, int GROUP>
+struct Q4Block {
+  static constexpr int kPer = kBlock / GROUP;
+  u32x4 q[RT];
+  float s[RT][kPer];
+  uint32_t z[RT][kPer];
+  __device__ __forceinline__ void load(const Q4View& w, int scale_type, const int (&row)[RT], int b,
+                                       int g, int cols, int groups) {
+    const int kw = b * kBlock + 32 * g;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      q[i] = kw < cols ? *reinterpret_cast<const u32x4*>(w.data + size_t(row[i]) * (cols / 2) + kw / 2)
+                       : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const size_t at = size_t(row[i]) * groups + min(b * kPer + p, groups - 1);
+        s[i][p] = q4_scale(w, scale_type, at);
+        z[i][p] = q4_zero(w, at);
+      }
+    }
+  }
+};
+
+// A few tiles of tokens: the slots' waves as in q4_few_kernel, each with its own blocks' parts straight
+// from the workspace; CT tiles of 16 tokens share the weights.
+template <bool GATE, int RT, int CT, int GROUP>
+__global__ void __launch_bounds__(64 * kSlots)
+q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
+                int row_groups) {
+  constexpr int NA = GATE ? 2 : 1, NT = NA * RT * CT;
+  constexpr int kPer = kBlock / GROUP;
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int tok_group = blockIdx.x / row_groups, row_group = blockIdx.x - tok_group * row_groups;
+  const int row0 = row_group * 16 * RT, tok0 = tok_group * 16 * CT;
+  const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
+  const int last_tile = (T - 1) / 16;
+  int row[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) row[i] = min(row0 + 16 * i + r, rows - 1);
+  f32x4 acc[NA][RT][CT];
+#pragma unroll
+  for (int n = 0; n < NA; ++n)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) acc[n][i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const Q4View w[2] = {w0, w1};
+  const int b1 = slot_block(wave + 1, blocks);
+  for (int b = slot_block(wave, blocks); b < b1; ++b) {
+    Q4Block<RT, GROUP> wb[NA];
+#pragma unroll
+    for (int n = 0; n < NA; ++n) wb[n].load(w[n], scale_type, row, b, g, cols, groups);
+    if constexpr (GROUP != 128) {
+#pragma unroll
+      for (int n = 0; n < NA; ++n)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) transpose4(wb[n].q[i]);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const size_t at = size_t(min(tok0 / 16 + c, last_tile)) * blocks + b;
+      const unsigned char* parts = x.parts + at * kPartBytes + lane * 16;
+      f16x8 hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        hi[j] = *reinterpret_cast<const f16x8*>(parts + j * 1024);
+        lo[j] = *reinterpret_cast<const f16x8*>(parts + 4096 + j * 1024);
+      }
+      const f32x4 back = *reinterpret_cast<const f32x4*>(x.back + at * 16 + 4 * g);
+#pragma unroll
+      for (int n = 0; n < NA; ++n)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int p = j * kPer / 4;
+            const f16x8 wq = unpack8(wb[n].q[i][j], wb[n].z[i][p]);
+            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[j], wq, part, 0, 0, 0);
+            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[j], wq, part, 0, 0, 0);
+            if ((j + 1) % (4 / kPer) == 0) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[n][i][c][e] = __builtin_fmaf(part[e], wb[n].s[i][p] * back[e], acc[n][i][c][e]);
+              part = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+          }
+        }
+    }
+  }
+  f32x4* sums = reinterpret_cast<f32x4*>(dyn);
+#pragma unroll
+  for (int n = 0; n < NA; ++n)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+        sums[(wave * NT + (n * RT + i) * CT + c) * 64 + lane] = acc[n][i][c];
+  __syncthreads();
+  for (int t = wave; t < RT * CT; t += kSlots) {
+    f32x4 v[NA];
+#pragma unroll
+    for (int n = 0; n < NA; ++n) {
+      v[n] = sums[(n * RT * CT + t) * 64 + lane];
+#pragma unroll
+      for (int sl = 1; sl < kSlots; ++sl) v[n] += sums[(sl * NT + n * RT * CT + t) * 64 + lane];
+    }
+    const int at = row0 + 16 * (t / CT) + r, tok1 = tok0 + 16 * (t % CT) + 4 * g;
+    if (at >= rows) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (tok1 + e >= T) break;
+      float o = v[0][e];
+      if constexpr (GATE) o = silu(o) * v[NA - 1][e];
+      q4_store(out, rows, tok1 + e, at, o);
+    }
+  }
+}
+
+// Prompts: 128 rows (64 of each matrix with GATE) x 128 tokens a workgroup, a wave 64 x 64 of them: 2 x 2
+// waves, one to a SIMD. The tokens' parts of a block reach LDS by DMA (64 KB, two stages, the next under
+// way while a block is multiplied); the weights go from memory to registers, where a wave unpacks them
+// once for its 64 tokens. All blocks are walked in turn, the slots' sums folded at their ends.
+template <bool GATE, int GROUP>
+__global__ void __launch_bounds__(256, 1)
+q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
+                int row_tiles, int tok_tiles) {
+  constexpr int NA = GATE ? 2 : 1, RT = 4, CT = 4, RM = RT / NA;  // RM: row tiles per matrix
+  constexpr int kPer = kBlock / GROUP;
+  constexpr int kStage = 8 * kPartBytes;
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15, wm = wave >> 1, wn = wave & 1;
+  int row_tile, tok_tile;
+  tile_of_block<GATE>(blockIdx.x, row_tiles, tok_tiles, row_tile, tok_tile);
+  const int row0 = (row_tile * 2 + wm) * 16 * RM, tok0 = tok_tile * 128;
+  const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
+  const int last_tile = (T - 1) / 16;
+  int row[RM];
+#pragma unroll
+  for (int i = 0; i < RM; ++i) row[i] = min(row0 + 16 * i + r, rows - 1);
+  const Q4View w[2] = {w0, w1};
+  const unsigned base = lds_address(dyn);
+  // Wave i brings token tiles 2i and 2i + 1 of a block: 16 transfers of 1 KB.
+  auto stage = [&](int b, int s) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const size_t at = size_t(min(tok_tile * 8 + 2 * wave + c, last_tile)) * blocks + b;
+      const unsigned char* src = x.parts + at * kPartBytes + lane * 16;
+      const unsigned to = base + s * kStage + (2 * wave + c) * kPartBytes;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dma16(src + j * 1024, to + j * 1024);
+    }
+  };
+  size_t tile_at[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) tile_at[c] = size_t(min(tok_tile * 8 + 4 * wn + c, last_tile)) * blocks;
+
+  f32x4 total[RT][CT], acc[RT][CT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      total[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  Q4Block<RM, GROUP> next[NA];
+  f32x4 next_back[CT];
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int n = 0; n < NA; ++n) next[n].load(w[n], scale_type, row, b, g, cols, groups);
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+      next_back[c] = *reinterpret_cast<const f32x4*>(x.back + (tile_at[c] + b) * 16 + 4 * g);
+  };
+  stage(0, 0);
+  fetch(0);
+  int b = 0;
+  for (int slot = 0; slot < kSlots; ++slot) {
+    const int b1 = slot_block(slot + 1, blocks);
+    for (; b < b1; ++b) {
+      wait_vmcnt<0>();
+      __syncthreads();
+      Q4Block<RM, GROUP> wb[NA];
+      f32x4 back[CT];
+#pragma unroll
+      for (int n = 0; n < NA; ++n) wb[n] = next[n];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) back[c] = next_back[c];
+      if (b + 1 < blocks) {
+        fetch(b + 1);
+        stage(b + 1, (b + 1) & 1);
+      }
+      if constexpr (GROUP != 128) {
+#pragma unroll
+        for (int n = 0; n < NA; ++n)
+#pragma unroll
+          for (int i = 0; i < RM; ++i) transpose4(wb[n].q[i]);
+      }
+      const unsigned char* parts = dyn + (b & 1) * kStage + 4 * wn * kPartBytes + lane * 16;
+      f32x4 part[RT][CT];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int p = j * kPer / 4;
+        f16x8 hi[CT], lo[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          hi[c] = *reinterpret_cast<const f16x8*>(parts + c * kPartBytes + j * 1024);
+          lo[c] = *reinterpret_cast<const f16x8*>(parts + c * kPartBytes + 4096 + j * 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          const Q4Block<RM, GROUP>& wi = wb[i / RM];
+          const f16x8 wq = unpack8(wi.q[i % RM][j], wi.z[i % RM][p]);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            if (j % (4 / kPer) == 0) part[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[c], wq, part[i][c], 0, 0, 0);
+          }
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+            part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[c], wq, part[i][c], 0, 0, 0);
+          if ((j + 1) % (4 / kPer) == 0) {
+            const float s = wi.s[i % RM][p];
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[i][c][e] = __builtin_fmaf(part[i][c][e], s * back[c][e], acc[i][c][e]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        total[i][c] = slot == 0 ? acc[i][c] : total[i][c] + acc[i][c];
+        acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    const int at = row0 + 16 * i + r;
+    if (at >= rows) continue;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = tok0 + (4 * wn + c) * 16 + 4 * g + e;
+        if (tok >= T) continue;
+        float o = total[i][c][e];
+        if constexpr (GATE) o = silu(o) * total[RM + i][c][e];
+        q4_store(out, rows, tok, at, o);
+      }
+  }
+}
+
 int check_matrix_q4(const ie_matrix_q4& m, const char* who) {
   if (!m.data || !m.scale || m.rows <= 0 || m.cols <= 0)
     return fail(IE_HIP_EINVAL, std::string(who) + ": empty weight matrix");
@@ -294,35 +598,87 @@ int check_matrix_q4(const ie_matrix_q4& m, const char* who) {
   return IE_HIP_OK;
 }
 
+// Tokens that a launch splits by itself; more are split once into the workspace.
+constexpr int kFewTokens = 16;
+
 struct Q4Launch {
   Q4Out out;
   const float* x;
   Q4View w0, w1;
   int scale_type, T, rows, cols;
+  Parts parts;
   hipStream_t stream;
+  const char* who;
 
+  int too_many() const { return fail(IE_HIP_EINVAL, std::string(who) + ": too many rows or tokens"); }
   template <bool GATE, int RT, int GROUP>
   int few() const {
     const int64_t row_groups = (int64_t(rows) + 16 * RT - 1) / (16 * RT);
-    const int64_t grid = row_groups * ((int64_t(T) + 15) / 16);
-    if (grid * 64 * kSlots > int64_t(UINT32_MAX)) return fail(IE_HIP_EINVAL, "matmul_q4: too many tiles");
-    hipLaunchKernelGGL((q4_few_kernel<GATE, RT, GROUP>), dim3(unsigned(grid)), dim3(64 * kSlots), 0,
+    if (row_groups * 64 * kSlots > int64_t(UINT32_MAX)) return too_many();
+    hipLaunchKernelGGL((q4_few_kernel<GATE, RT, GROUP>), dim3(unsigned(row_groups)), dim3(64 * kSlots), 0,
                        stream, out, x, w0, w1, scale_type, T, rows, cols, int(row_groups));
     return IE_HIP_OK;
   }
+  template <bool GATE, int RT, int CT, int GROUP>
+  int slots() const {
+    constexpr int kLds = kSlots * (GATE ? 2 : 1) * RT * CT * 1024;
+    const auto kernel = q4_slots_kernel<GATE, RT, CT, GROUP>;
+    if (kLds > 64 * 1024) {
+      static const hipError_t attr = hipFuncSetAttribute(
+          reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+      if (int rc = check_hip(attr, "hipFuncSetAttribute(q4)")) return rc;
+    }
+    const int64_t row_groups = (int64_t(rows) + 16 * RT - 1) / (16 * RT);
+    const int64_t grid = row_groups * ((int64_t(T) + 16 * CT - 1) / (16 * CT));
+    if (grid * 64 * kSlots > int64_t(UINT32_MAX)) return too_many();
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(64 * kSlots), kLds, stream, out, parts, w0, w1,
+                       scale_type, T, rows, cols, int(row_groups));
+    return IE_HIP_OK;
+  }
   template <bool GATE, int GROUP>
-  int few_rows() const {
-    const int64_t tiles = (int64_t(rows) + 15) / 16;
-    const int cus = device_compute_units();
-    if (tiles >= 8 * cus) return few<GATE, 4, GROUP>();
-    if (tiles >= 4 * cus) return few<GATE, 2, GROUP>();
-    return few<GATE, 1, GROUP>();
+  int tiles() const {
+    constexpr int kLds = 2 * 8 * kPartBytes, kRows = GATE ? 64 : 128;
+    const auto kernel = q4_tiles_kernel<GATE, GROUP>;
+    static const hipError_t attr = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (int rc = check_hip(attr, "hipFuncSetAttribute(q4)")) return rc;
+    const int64_t row_tiles = (int64_t(rows) + kRows - 1) / kRows, tok_tiles = (int64_t(T) + 127) / 128;
+    if (row_tiles * tok_tiles * 256 > int64_t(UINT32_MAX)) return too_many();
+    hipLaunchKernelGGL(kernel, dim3(unsigned(row_tiles * tok_tiles)), dim3(256), kLds, stream, out, parts,
+                       w0, w1, scale_type, T, rows, cols, int(row_tiles), int(tok_tiles));
+    return IE_HIP_OK;
+  }
+  template <bool GATE, int GROUP>
+  int run() const {
+    const int64_t row_tiles = (int64_t(rows) + 15) / 16;
+    const int64_t cus = device_compute_units();
+    if (T <= kFewTokens) {
+      if (row_tiles >= 8 * cus) return few<GATE, 4, GROUP>();
+      if (row_tiles >= 4 * cus) return few<GATE, 2, GROUP>();
+      return few<GATE, 1, GROUP>();
+    }
+    const int64_t tok_tiles = (int64_t(T) + 15) / 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
+    if (tok_tiles * blocks * 256 > int64_t(UINT32_MAX)) return too_many();
+    hipLaunchKernelGGL(q4_split_kernel<GROUP == 128>, dim3(unsigned(tok_tiles * blocks)), dim3(256), 0,
+                       stream, parts, x, T, cols, int(blocks));
+    const int64_t big = ((int64_t(rows) + (GATE ? 63 : 127)) / (GATE ? 64 : 128)) * ((int64_t(T) + 127) / 128);
+    if (2 * big >= cus) return tiles<GATE, GROUP>();
+    if (T <= 32) return row_tiles >= 4 * cus ? slots<GATE, 2, 2, GROUP>() : slots<GATE, 1, 2, GROUP>();
+    if constexpr (!GATE)
+      if (row_tiles >= 2 * cus) return slots<GATE, 2, 4, GROUP>();
+    return slots<GATE, 1, 4, GROUP>();
   }
   template <bool GATE>
   int run(int group) const {
-    return group == 128 ? few_rows<GATE, 128>() : group == 64 ? few_rows<GATE, 64>() : few_rows<GATE, 32>();
+    return group == 128 ? run<GATE, 128>() : group == 64 ? run<GATE, 64>() : run<GATE, 32>();
   }
 };
+
+Parts parts_of(void* workspace, int T, int cols) {
+  unsigned char* base = static_cast<unsigned char*>(workspace);
+  const size_t n = part_tiles(T) * ((size_t(cols) + kBlock - 1) / kBlock);
+  return Parts{base, reinterpret_cast<float*>(base + n * kPartBytes)};
+}
 
 int launch_q4(bool gate, float* y, const float* x, const ie_matrix_q4& w, const ie_matrix_q4* w2,
               const float* bias, int T, int accumulate, void* workspace, hipStream_t stream,
@@ -357,7 +713,9 @@ int launch_q4(bool gate, float* y, const float* x, const ie_matrix_q4& w, const 
                         T,
                         w.rows,
                         w.cols,
-                        stream};
+                        parts_of(workspace, T, w.cols),
+                        stream,
+                        who};
   if (int rc = gate ? launch.run<true>(w.group) : launch.run<false>(w.group)) return rc;
   return check_launch(who);
 }
@@ -368,9 +726,8 @@ int launch_q4(bool gate, float* y, const float* x, const ie_matrix_q4& w, const 
 using namespace iehip;
 
 extern "C" size_t ie_hip_matmul_q4_workspace_bytes(int T, int cols) {
-  (void)T;
-  (void)cols;
-  return 0;
+  if (T <= kFewTokens || cols <= 0) return 0;
+  return part_tiles(T) * ((size_t(cols) + kBlock - 1) / kBlock) * (kPartBytes + 64);
 }
 
 extern "C" int ie_hip_matmul_q4(float* y, const float* x, ie_matrix_q4 w, const float* bias, int T,
