@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kBlock = 128;  // columns that share an activation scale: 4 products of 32
 constexpr int kSlots = 8;
+constexpr int kMaxCols = 1 << 24;  // a tile's byte offsets from its first row fit 32 bits
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -38,36 +39,33 @@ __host__ __device__ __forceinline__ int slot_block(int i, int n) { return int(in
 // One 4-bit matrix as a kernel sees it.
 struct Q4View {
   const uint8_t* data;
-  const void* scale;
-  const uint8_t* zero;
+  const uint8_t* scale;
+  const uint8_t* zero;  // null: 8 everywhere
 };
+__device__ const uint8_t kEight[4] = {8, 8, 8, 8};
 
-// The scale of (row, group) and the pair of f16 constants that take a weight's zero point off.
-__device__ __forceinline__ float q4_scale(const Q4View& w, int type, size_t at) {
-  if (type == IE_KV_F32) return static_cast<const float*>(w.scale)[at];
-  const uint16_t b = static_cast<const uint16_t*>(w.scale)[at];
-  return type == IE_KV_F16 ? f16_bits_to_f32(b) : bf16_bits_to_f32(b);
-}
-__device__ __forceinline__ uint32_t q4_zero(const Q4View& w, size_t at) {
-  return w.zero ? w.zero[at] : 8u;
+// A group's zero point as the two pairs of f16 constants that take it off its weights.
+struct Q4Zero {
+  f16x2 low, high;  // 1024 + z; -(64 + z)
+};
+__device__ __forceinline__ Q4Zero q4_zero(uint32_t z) {
+  const _Float16 h = static_cast<_Float16>(-64.0f - static_cast<float>(z));
+  return Q4Zero{__builtin_bit_cast(f16x2, 0x64006400u + z * 0x10001u), f16x2{h, h}};
 }
 
 // 8 weights of a word, less their zero point, as f16: element order 0, 4, 1, 5, 2, 6, 3, 7.
 // A nibble in the low bits of an f16 of 1,024 reads 1024 + q; one four bits up reads 1024 + 16 q,
-// which an fma with 1/16 brings down: every step is exact. (4 + 1 bit operations and 4 packed ones
-// for 8 weights.)
-__device__ __forceinline__ f16x8 unpack8(uint32_t w, uint32_t zero) {
-  const uint32_t base = 0x64006400u;
-  auto pair = [](uint32_t v) { return __builtin_bit_cast(f16x2, v); };
-  const f16x2 z1024 = pair(base + zero * 0x10001u);                           // 1024 + z
-  const _Float16 z = static_cast<_Float16>(-64.0f - static_cast<float>(zero));  // -(64 + z)
-  const f16x2 z64 = {z, z};
-  const f16x2 sixteenth = {_Float16(0.0625f), _Float16(0.0625f)};
+// which an fma with 1/16 brings down: every step is exact, 9 instructions for 8 weights.
+__device__ __forceinline__ f16x8 unpack8(uint32_t w, const Q4Zero& z) {
+  uint32_t base = 0x64006400u;
+  asm("" : "+v"(base));  // in a register: of two literals the compiler makes an and and an or
   const uint32_t h = w >> 8;
-  const f16x2 a = pair((w & 0x000F000Fu) | base) - z1024;
-  const f16x2 b = __builtin_elementwise_fma(pair((w & 0x00F000F0u) | base), sixteenth, z64);
-  const f16x2 c = pair((h & 0x000F000Fu) | base) - z1024;
-  const f16x2 d = __builtin_elementwise_fma(pair((h & 0x00F000F0u) | base), sixteenth, z64);
+  auto pair = [&](uint32_t v, uint32_t mask) { return __builtin_bit_cast(f16x2, (v & mask) | base); };
+  const f16x2 sixteenth = {_Float16(0.0625f), _Float16(0.0625f)};
+  const f16x2 a = pair(w, 0x000F000Fu) - z.low;
+  const f16x2 b = __builtin_elementwise_fma(pair(w, 0x00F000F0u), sixteenth, z.high);
+  const f16x2 c = pair(h, 0x000F000Fu) - z.low;
+  const f16x2 d = __builtin_elementwise_fma(pair(h, 0x00F000F0u), sixteenth, z.high);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
@@ -107,15 +105,156 @@ __device__ __forceinline__ void split8(const float (&x)[8], float factor, f16x8&
   }
 }
 
-// Where the part of columns 8 k8 .. 8 k8 + 7 of a block stands in LDS: 16 bytes per (step, lane
-// group, token), tokens permuted by k8 so that the 16 lanes that write a token's block hit every bank.
-// WIDE (groups of 128): step j holds columns 32 g + 8 j of lane group g, as the weights are loaded;
-// otherwise step j is columns 32 j .. 32 j + 31 and the weights are transposed to it.
+// Columns 8 k8 .. 8 k8 + 7 of a block belong to step `step` of lane group g of the products. WIDE
+// (groups of 128): step j holds columns 32 g + 8 j of lane group g, as the weights are loaded; otherwise
+// step j is columns 32 j .. 32 j + 31 and the weights are transposed to it.
 template <bool WIDE>
-__device__ __forceinline__ int part_slot(int step, int g, int tok) {
-  const int k8 = WIDE ? 4 * g + step : 4 * step + g;
-  return step * 64 + 16 * g + (tok ^ k8);
+__device__ __forceinline__ int k8_of(int step, int g) {
+  return WIDE ? 4 * g + step : 4 * step + g;
 }
+
+// A block's parts in LDS: 16 bytes per (k8, token), hi then lo, TP token places. Of 16 places they are
+// permuted by k8, so that the 16 lanes that write a token's block hit every bank.
+template <int TP>
+struct Places {
+  static constexpr int kHalf = 16 * TP * 16, kBytes = 2 * kHalf;
+  __device__ __forceinline__ static int at(int k8, int tok) {
+    return (k8 * TP + (TP == 16 ? tok ^ k8 : tok)) * 16;
+  }
+};
+
+// A lane's 8 activations of a (token, block), split among the 16 lanes that hold the block.
+__device__ __forceinline__ float split_lane(const float (&v)[8], f16x8& hi, f16x8& lo) {
+  uint32_t largest = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) largest = max(largest, finite_bits(v[i]));
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) largest = max(largest, uint32_t(__shfl_xor(int(largest), off, 64)));
+  float factor, back;
+  block_scale(largest, factor, back);
+  split8(v, factor, hi, lo);
+  return back;
+}
+__device__ __forceinline__ void load8(float (&v)[8], const float* src, bool in) {
+  const float4* p = reinterpret_cast<const float4*>(src);
+  const float4 a = in ? p[0] : make_float4(0.f, 0.f, 0.f, 0.f);
+  const float4 b = in ? p[1] : make_float4(0.f, 0.f, 0.f, 0.f);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// A lane's rows of RT row tiles from row0 on: byte offsets from the first of them, which is uniform.
+template <int RT, int GROUP, bool S32>
+struct Q4Rows {
+  static constexpr int kPer = kBlock / GROUP, kSize = S32 ? 4 : 2;
+  const uint8_t *data, *scale, *zero;
+  uint32_t q[RT], s[RT], z[RT];
+  int last_word, groups, step;
+  bool bf16;
+  __device__ __forceinline__ Q4Rows(const Q4View& w, int scale_type, int row0, int rows, int cols, int r) {
+    const int first = min(row0, rows - 1);
+    groups = (cols + GROUP - 1) / GROUP;
+    step = w.zero ? 1 : 0;
+    bf16 = scale_type == IE_KV_BF16;
+    last_word = cols / 2 - 16;
+    data = w.data + size_t(first) * (cols / 2);
+    scale = w.scale + size_t(first) * groups * kSize;
+    zero = w.zero ? w.zero + size_t(first) * groups : kEight;
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const uint32_t row = min(16 * i + r, rows - 1 - first);
+      q[i] = row * (cols / 2);
+      s[i] = row * groups * kSize;
+      z[i] = row * groups * step;
+    }
+  }
+};
+
+// A lane's weights of one block, with the scale and zero point of the group that step g of the block
+// falls into (so that the four lane groups hold a block's between them). Lanes past the last column take
+// the columns before it: their activations are 0.
+template <int RT, int GROUP, bool S32>
+struct Q4Block {
+  static constexpr int kPer = kBlock / GROUP;
+  u32x4 q[RT];
+  uint32_t s[RT], z[RT];
+  __device__ __forceinline__ void load(const Q4Rows<RT, GROUP, S32>& w, int b, int g) {
+    const uint32_t k = min(b * (kBlock / 2) + 16 * g, w.last_word);
+    const uint32_t group = min(b * kPer + g * kPer / 4, w.groups - 1);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      q[i] = *reinterpret_cast<const u32x4*>(w.data + (w.q[i] + k));
+      const uint8_t* at = w.scale + (w.s[i] + group * w.kSize);
+      if constexpr (S32)
+        s[i] = *reinterpret_cast<const uint32_t*>(at);
+      else
+        s[i] = *reinterpret_cast<const uint16_t*>(at);
+      z[i] = w.zero[w.z[i] + group * w.step];
+    }
+  }
+};
+
+// One of its row tiles ready to multiply: the words' order and each step's scale and zero point.
+template <int GROUP, bool S32>
+struct Q4Tile {
+  static constexpr int kPer = kBlock / GROUP;
+  u32x4 q;
+  float scale[kPer];
+  Q4Zero zero[kPer];
+  __device__ __forceinline__ void set(int p, uint32_t s, uint32_t z, bool bf16) {
+    if constexpr (S32)
+      scale[p] = __uint_as_float(s);
+    else
+      scale[p] = bf16 ? __uint_as_float(s << 16) : f16_bits_to_f32(uint16_t(s));
+    zero[p] = q4_zero(z);
+  }
+  __device__ __forceinline__ Q4Tile(const u32x4& words, const uint32_t (&s)[kPer], const uint32_t (&z)[kPer],
+                                    bool bf16)
+      : q(words) {
+    if constexpr (kPer > 1) transpose4(q);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) set(p, s[p], z[p], bf16);
+  }
+  template <int RT>
+  __device__ __forceinline__ Q4Tile(const Q4Block<RT, GROUP, S32>& b, int i, bool bf16) : q(b.q[i]) {
+    u32x4 s = u32x4(b.s[i]), z = u32x4(b.z[i]);
+    if constexpr (kPer > 1) {
+      transpose4(q);
+      if constexpr (S32) {
+        transpose4(s);
+        transpose4(z);
+      } else {
+        s = u32x4(b.s[i] | b.z[i] << 16);
+        transpose4(s);
+        z = s >> 16;
+        s &= 0xFFFF;
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) set(p, s[p * 4 / kPer], z[p * 4 / kPer], bf16);
+  }
+  __device__ __forceinline__ f16x8 weights(int step) const { return unpack8(q[step], zero[step * kPer / 4]); }
+  __device__ __forceinline__ void unpack(f16x8 (&wq)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) wq[j] = weights(j);
+  }
+  // The tile times one tile of tokens, added to acc group by group.
+  __device__ __forceinline__ void multiply(const f16x8 (&wq)[4], const f16x8 (&hi)[4], const f16x8 (&lo)[4],
+                                           const f32x4& back, f32x4& acc) const {
+    f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      part = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[j], wq[j], part, 0, 0, 0);
+      part = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[j], wq[j], part, 0, 0, 0);
+      if ((j + 1) % (4 / kPer) == 0) {
+        const float sc = scale[j * kPer / 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(part[e], sc * back[e], acc[e]);
+        part = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  }
+};
 
 struct Q4Out {
   float* y;
@@ -137,143 +276,195 @@ __device__ __forceinline__ void q4_store(const Q4Out& o, int rows, int tok, int 
   *dst = v;
 }
 
-// A workgroup: RT tiles of 16 rows (per matrix) by one tile of 16 tokens; wave i takes slot i. A wave
-// splits its own blocks of activations through 8 KB of LDS of its own, so no wave waits for another
-// before the slots are added.
-template <bool GATE, int RT, int GROUP>
+// Global -> LDS transfers of 4, 2 or 1 bytes a lane, widened to the lane's word at lds + 4 lane; as dma16.
+template <int BYTES>
+__device__ __forceinline__ void dma_word(const void* base, unsigned offset, unsigned lds) {
+  if constexpr (BYTES == 4)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(lds)
+                 : "memory", "m0");
+  else if constexpr (BYTES == 2)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(lds)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// A barrier for data in LDS that leaves loads from memory under way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// LDS of q4_few_kernel: two stages a wave, the slots' sums, the activations' parts and powers.
+template <bool GATE, int GROUP, int TP, int SB, bool SPLIT>
+struct FewShape {
+  static constexpr int NA = GATE ? 2 : 1, kPer = kBlock / GROUP;
+  static constexpr int kScales = (SB * kPer + 3) / 4;  // transfers of 4 groups' scales
+  static constexpr int kUnit = SB * 1024 + kScales * 512, kStage = NA * kUnit;
+  static constexpr int kLoads = NA * (SB + 2 * kScales);
+  static constexpr int kSums = kSlots * 2 * kStage, kParts = kSums + (SPLIT ? kSlots * NA * 1024 : 0);
+  static constexpr int64_t bytes(int64_t blocks) { return kParts + blocks * (Places<TP>::kBytes + 4 * TP); }
+};
+
+// Up to 16 tokens whose parts fit LDS beside the rest: a workgroup splits them once, then its waves stream
+// weights past them through two stages of LDS each: SB blocks of 16 rows (of each matrix) by DMA, 64 SB
+// contiguous bytes of a row a transfer, the next stage under way while one is multiplied. SPLIT: a
+// workgroup takes row tiles in turn, wave i slot i, and the slots are added through LDS. Otherwise (row
+// tiles enough for every wave) a wave takes row tiles of its own, all blocks, folding slots as it passes
+// their ends, and waits for nobody. TP: token places, 1, 4 or 16.
+// Loads straight to registers touch 16 rows 64 bytes at a time, which bounds them (8,192 x 8,192 at 1
+// token: 22 us so).
+template <bool GATE, int GROUP, bool S32, int TP, int SB, bool SPLIT>
 __global__ void __launch_bounds__(64 * kSlots)
-q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int scale_type, int T,
-              int rows, int cols, int row_groups) {
-  constexpr int NA = GATE ? 2 : 1, NT = NA * RT;
-  constexpr bool WIDE = GROUP == 128;
-  constexpr int kPer = kBlock / GROUP;  // groups of a block
-  constexpr int kStage = 8192 + 64;
-  constexpr int kLds = kSlots * kStage > kSlots * NT * 1024 ? kSlots * kStage : kSlots * NT * 1024;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
+q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int scale_type, int T, int rows,
+              int cols, int row_tiles) {
+  using F = FewShape<GATE, GROUP, TP, SB, SPLIT>;
+  using P = Places<TP>;
+  constexpr int NA = F::NA, kPer = F::kPer, kSize = S32 ? 4 : 2, kWide = 4 * SB;  // kWide: words x 4 of a row
+  constexpr int kShift = SB == 4 ? 0 : SB == 2 ? 1 : 2;
+  constexpr bool WIDE = GROUP == kBlock;
+  extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int tok_tile = blockIdx.x / row_groups, row_group = blockIdx.x - tok_tile * row_groups;
-  const int row0 = row_group * 16 * RT, tok0 = tok_tile * 16;
-  const int nt = min(16, T - tok0);
   const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
-  unsigned char* stage = lds + wave * kStage;
-  float* back_of = reinterpret_cast<float*>(stage + 8192);
-  const Q4View w[2] = {w0, w1};
+  const int b0 = SPLIT ? slot_block(wave, blocks) : 0, b1 = SPLIT ? slot_block(wave + 1, blocks) : blocks;
+  const int first = SPLIT ? blockIdx.x : blockIdx.x * kSlots + wave;
+  const int hop = SPLIT ? gridDim.x : gridDim.x * kSlots;
+  const bool bf16 = scale_type == IE_KV_BF16;
+  unsigned char* ring = dyn + wave * 2 * F::kStage;
+  const unsigned ring_lds = lds_address(ring);
+  unsigned char* parts = dyn + F::kParts;
+  float* backs = reinterpret_cast<float*>(parts + size_t(blocks) * P::kBytes);
 
-  f32x4 acc[NA][RT];
-#pragma unroll
-  for (int n = 0; n < NA; ++n)
-#pragma unroll
-    for (int i = 0; i < RT; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int row[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) row[i] = min(row0 + 16 * i + r, rows - 1);
-
-  const int b1 = slot_block(wave + 1, blocks);
-  for (int b = slot_block(wave, blocks); b < b1; ++b) {
-    const int kw = b * kBlock + 32 * g;  // this lane's 32 columns
-    u32x4 q[NA][RT];
-    float s[NA][RT][kPer];
-    uint32_t z[NA][RT][kPer];
-#pragma unroll
-    for (int n = 0; n < NA; ++n)
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        q[n][i] = kw < cols ? *reinterpret_cast<const u32x4*>(w[n].data + size_t(row[i]) * (cols / 2) + kw / 2)
-                            : u32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int p = 0; p < kPer; ++p) {
-          const size_t at = size_t(row[i]) * groups + min(b * kPer + p, groups - 1);
-          s[n][i][p] = q4_scale(w[n], scale_type, at);
-          z[n][i][p] = q4_zero(w[n], at);
-        }
-      }
-    // Split the block's activations: 16 lanes per token, 8 columns each.
-    for (int t = lane >> 4; t < nt; t += 4) {
-      const int k8 = lane & 15, k = b * kBlock + 8 * k8;
-      float v[8];
-      uint32_t largest = 0;
-      const float4* src = reinterpret_cast<const float4*>(x + size_t(tok0 + t) * cols + k);
-      const float4 v0 = k < cols ? src[0] : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 v1 = k < cols ? src[1] : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w;
-      v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) largest = max(largest, finite_bits(v[i]));
-#pragma unroll
-      for (int off = 8; off > 0; off >>= 1) largest = max(largest, uint32_t(__shfl_xor(int(largest), off, 64)));
-      float factor, back;
-      block_scale(largest, factor, back);
-      f16x8 hi, lo;
-      split8(v, factor, hi, lo);
-      const int step = WIDE ? k8 & 3 : k8 >> 2, kg = WIDE ? k8 >> 2 : k8 & 3;
-      const int at = part_slot<WIDE>(step, kg, t) * 16;
-      *reinterpret_cast<f16x8*>(stage + at) = hi;
-      *reinterpret_cast<f16x8*>(stage + 4096 + at) = lo;
-      if (k8 == 0) back_of[t] = back;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    f16x8 hi[4], lo[4];
-    const int tr = min(r, nt - 1);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int at = part_slot<WIDE>(j, g, tr) * 16;
-      hi[j] = *reinterpret_cast<const f16x8*>(stage + at);
-      lo[j] = *reinterpret_cast<const f16x8*>(stage + 4096 + at);
-    }
-    f32x4 back;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) back[e] = back_of[min(4 * g + e, nt - 1)];
-#pragma unroll
-    for (int n = 0; n < NA; ++n)
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if constexpr (!WIDE) transpose4(q[n][i]);
-        f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int p = j * kPer / 4;
-          const f16x8 wq = unpack8(q[n][i][j], z[n][i][p]);
-          part = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[j], wq, part, 0, 0, 0);
-          part = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[j], wq, part, 0, 0, 0);
-          if ((j + 1) % (4 / kPer) == 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              acc[n][i][e] = __builtin_fmaf(part[e], s[n][i][p] * back[e], acc[n][i][e]);
-            part = f32x4{0.f, 0.f, 0.f, 0.f};
-          }
-        }
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
-  // The slots' tiles through LDS, added in slot order.
-  __syncthreads();
-  f32x4* sums = reinterpret_cast<f32x4*>(lds);
-#pragma unroll
-  for (int n = 0; n < NA; ++n)
-#pragma unroll
-    for (int i = 0; i < RT; ++i) sums[(wave * NT + n * RT + i) * 64 + lane] = acc[n][i];
-  __syncthreads();
-  for (int i = wave; i < RT; i += kSlots) {
-    f32x4 v[NA];
+  auto issue = [&](int tile, int b, int stage) {
+    const int row0 = tile * 16, last_row = rows - 1 - row0;
 #pragma unroll
     for (int n = 0; n < NA; ++n) {
-      v[n] = sums[(n * RT + i) * 64 + lane];
+      const Q4View& w = n ? w1 : w0;
+      const unsigned to = ring_lds + stage * F::kStage + n * F::kUnit;
+      const uint8_t* data = w.data + size_t(row0) * (cols / 2);
 #pragma unroll
-      for (int sl = 1; sl < kSlots; ++sl) v[n] += sums[(sl * NT + n * RT + i) * 64 + lane];
+      for (int i = 0; i < SB; ++i) {
+        const int row = 64 / kWide * i + lane / kWide;
+        const int word = min(4 * b + ((lane % kWide) ^ (row >> kShift)), cols / 32 - 1);
+        dma16_at(data, uint32_t(min(row, last_row)) * (cols / 2) + word * 16, to + i * 1024);
+      }
+      const uint32_t step = w.zero ? 1 : 0;
+      const uint8_t* scale = w.scale + size_t(row0) * groups * kSize;
+      const uint8_t* zero = w.zero ? w.zero + size_t(row0) * groups : kEight;
+#pragma unroll
+      for (int p = 0; p < F::kScales; ++p) {
+        const uint32_t at = uint32_t(min(r, last_row)) * groups + min(b * kPer + 4 * p + g, groups - 1);
+        dma_word<kSize>(scale, at * kSize, to + SB * 1024 + p * 256);
+        dma_word<1>(zero, at * step, to + SB * 1024 + (F::kScales + p) * 256);
+      }
     }
-    const int at = row0 + 16 * i + r;
+  };
+  int stage = 0;
+  if (first < row_tiles && b0 < b1) issue(first, b0, 0);
+  for (int u = threadIdx.x >> 4; u < blocks * T; u += 32) {
+    const int b = u / T, tok = u - b * T, k8 = r, k = b * kBlock + 8 * k8;
+    float v[8];
+    load8(v, x + size_t(tok) * cols + (k < cols ? k : 0), k < cols);
+    f16x8 hi, lo;
+    const float back = split_lane(v, hi, lo);
+    unsigned char* to = parts + b * P::kBytes + P::at(k8, tok);
+    *reinterpret_cast<f16x8*>(to) = hi;
+    *reinterpret_cast<f16x8*>(to + P::kHalf) = lo;
+    if (k8 == 0) backs[b * TP + tok] = back;
+  }
+  lds_barrier();
+  for (int tile = first; tile < row_tiles; tile += hop) {
+    f32x4 total[NA], acc[NA];
+#pragma unroll
+    for (int n = 0; n < NA; ++n) total[n] = acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int slot = 0;
+    for (int b = b0; b < b1; b += SB) {
+      wait_lds();  // the other stage has been read
+      if (b + SB < b1) {
+        issue(tile, b + SB, stage ^ 1);
+        wait_vmcnt<F::kLoads>();
+      } else if (tile + hop < row_tiles) {
+        issue(tile + hop, b0, stage ^ 1);
+        wait_vmcnt<F::kLoads>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      asm volatile("" ::: "memory");
+      const unsigned char* from = ring + stage * F::kStage;
+      stage ^= 1;
+#pragma unroll
+      for (int sb = 0; sb < SB; ++sb) {
+        if (b + sb >= b1) break;
+        const unsigned char* at = parts + size_t(b + sb) * P::kBytes;
+        f16x8 hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned char* part = at + P::at(k8_of<WIDE>(j, g), TP == 1 ? 0 : min(r, T - 1));
+          hi[j] = *reinterpret_cast<const f16x8*>(part);
+          lo[j] = *reinterpret_cast<const f16x8*>(part + P::kHalf);
+        }
+        f32x4 back;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) back[e] = backs[(b + sb) * TP + (TP == 1 ? 0 : min(4 * g + e, T - 1))];
+#pragma unroll
+        for (int n = 0; n < NA; ++n) {
+          const unsigned char* unit = from + n * F::kUnit;
+          const u32x4 q = *reinterpret_cast<const u32x4*>(unit + (r * kWide + ((4 * sb + g) ^ (r >> kShift))) * 16);
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(unit + SB * 1024);
+          uint32_t sc[kPer], ze[kPer];
+#pragma unroll
+          for (int p = 0; p < kPer; ++p) {
+            const int in = sb * kPer + p;
+            sc[p] = words[in / 4 * 64 + in % 4 * 16 + r];
+            if constexpr (!S32) sc[p] &= 0xFFFFu;
+            ze[p] = words[(F::kScales + in / 4) * 64 + in % 4 * 16 + r] & 0xFFu;
+          }
+          const Q4Tile<GROUP, S32> t(q, sc, ze, bf16);
+          f16x8 wq[4];
+          t.unpack(wq);
+          t.multiply(wq, hi, lo, back, acc[n]);
+        }
+        if constexpr (!SPLIT)
+          while (slot < kSlots && slot_block(slot + 1, blocks) <= b + sb + 1) {
+#pragma unroll
+            for (int n = 0; n < NA; ++n) {
+              total[n] += acc[n];
+              acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            ++slot;
+          }
+      }
+    }
+    if constexpr (SPLIT) {
+      f32x4* sums = reinterpret_cast<f32x4*>(dyn + F::kSums);
+      lds_barrier();  // the last tile's sums have been read
+#pragma unroll
+      for (int n = 0; n < NA; ++n) sums[(wave * NA + n) * 64 + lane] = acc[n];
+      lds_barrier();
+      if (wave != 0) continue;
+#pragma unroll
+      for (int n = 0; n < NA; ++n)
+#pragma unroll
+        for (int sl = 0; sl < kSlots; ++sl) total[n] += sums[(sl * NA + n) * 64 + lane];
+    }
+    const int at = tile * 16 + r;
     if (at >= rows) continue;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int tok = 4 * g + e;
-      if (tok >= nt) break;
-      float o = v[0][e];
-      if constexpr (GATE) o = silu(o) * v[NA - 1][e];
-      q4_store(out, rows, tok0 + tok, at, o);
+      if (tok >= T) break;
+      float o = total[0][e];
+      if constexpr (GATE) o = silu(o) * total[NA - 1][e];
+      q4_store(out, rows, tok, at, o);
     }
   }
 }
@@ -296,22 +487,11 @@ q4_split_kernel(Parts out, const float* __restrict__ x, int T, int cols, int blo
   const size_t tile = blockIdx.x / blocks, b = blockIdx.x - tile * blocks;
   const int t = threadIdx.x >> 4, k8 = threadIdx.x & 15, k = int(b) * kBlock + 8 * k8;
   const size_t tok = tile * 16 + t;
-  float v[8] = {};
-  if (tok < size_t(T) && k < cols) {
-    const float4* src = reinterpret_cast<const float4*>(x + tok * cols + k);
-    const float4 v0 = src[0], v1 = src[1];
-    v[0] = v0.x; v[1] = v0.y; v[2] = v0.z; v[3] = v0.w;
-    v[4] = v1.x; v[5] = v1.y; v[6] = v1.z; v[7] = v1.w;
-  }
-  uint32_t largest = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) largest = max(largest, finite_bits(v[i]));
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) largest = max(largest, uint32_t(__shfl_xor(int(largest), off, 64)));
-  float factor, back;
-  block_scale(largest, factor, back);
+  const bool in = tok < size_t(T) && k < cols;
+  float v[8];
+  load8(v, x + (in ? tok * cols + k : 0), in);
   f16x8 hi, lo;
-  split8(v, factor, hi, lo);
+  const float back = split_lane(v, hi, lo);
   const int step = WIDE ? k8 & 3 : k8 >> 2, g = WIDE ? k8 >> 2 : k8 & 3;
   unsigned char* to = out.parts + (tile * blocks + b) * kPartBytes + (step * 64 + 16 * g + t) * 16;
   *reinterpret_cast<f16x8*>(to) = hi;
@@ -319,49 +499,21 @@ q4_split_kernel(Parts out, const float* __restrict__ x, int T, int cols, int blo
   if (k8 == 0) out.back[(tile * blocks + b) * 16 + t] = back;
 }
 
-// A lane's weights, scales and zero points of one block.
-template <int RT, int GROUP>
-struct Q4Block {
-  static constexpr int kPer = kBlock / GROUP;
-  u32x4 q[RT];
-  float s[RT][kPer];
-  uint32_t z[RT][kPer];
-  __device__ __forceinline__ void load(const Q4View& w, int scale_type, const int (&row)[RT], int b,
-                                       int g, int cols, int groups) {
-    const int kw = b * kBlock + 32 * g;
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      q[i] = kw < cols ? *reinterpret_cast<const u32x4*>(w.data + size_t(row[i]) * (cols / 2) + kw / 2)
-                       : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int p = 0; p < kPer; ++p) {
-        const size_t at = size_t(row[i]) * groups + min(b * kPer + p, groups - 1);
-        s[i][p] = q4_scale(w, scale_type, at);
-        z[i][p] = q4_zero(w, at);
-      }
-    }
-  }
-};
-
 // A few tiles of tokens: the slots' waves as in q4_few_kernel, each with its own blocks' parts straight
 // from the workspace; CT tiles of 16 tokens share the weights.
-template <bool GATE, int RT, int CT, int GROUP>
+template <bool GATE, int RT, int CT, int GROUP, bool S32>
 __global__ void __launch_bounds__(64 * kSlots)
 q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
                 int row_groups) {
   constexpr int NA = GATE ? 2 : 1, NT = NA * RT * CT;
-  constexpr int kPer = kBlock / GROUP;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
   const int tok_group = blockIdx.x / row_groups, row_group = blockIdx.x - tok_group * row_groups;
   const int row0 = row_group * 16 * RT, tok0 = tok_group * 16 * CT;
-  const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
+  const int blocks = (cols + kBlock - 1) / kBlock;
   const int last_tile = (T - 1) / 16;
-  int row[RT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) row[i] = min(row0 + 16 * i + r, rows - 1);
   f32x4 acc[NA][RT][CT];
 #pragma unroll
   for (int n = 0; n < NA; ++n)
@@ -369,49 +521,45 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int c = 0; c < CT; ++c) acc[n][i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const Q4View w[2] = {w0, w1};
-  const int b1 = slot_block(wave + 1, blocks);
-  for (int b = slot_block(wave, blocks); b < b1; ++b) {
-    Q4Block<RT, GROUP> wb[NA];
+  const Q4Rows<RT, GROUP, S32> w[2] = {{w0, scale_type, row0, rows, cols, r},
+                                       {GATE ? w1 : w0, scale_type, row0, rows, cols, r}};
+  const int b0 = slot_block(wave, blocks), b1 = slot_block(wave + 1, blocks);
+  Q4Block<RT, GROUP, S32> next[NA];
+  if (b0 < b1) {
 #pragma unroll
-    for (int n = 0; n < NA; ++n) wb[n].load(w[n], scale_type, row, b, g, cols, groups);
-    if constexpr (GROUP != 128) {
+    for (int n = 0; n < NA; ++n) next[n].load(w[n], b0, g);
+  }
+  for (int b = b0; b < b1; ++b) {
+    Q4Block<RT, GROUP, S32> wb[NA];
 #pragma unroll
-      for (int n = 0; n < NA; ++n)
+    for (int n = 0; n < NA; ++n) wb[n] = next[n];
+    if (b + 1 < b1) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i) transpose4(wb[n].q[i]);
+      for (int n = 0; n < NA; ++n) next[n].load(w[n], b + 1, g);
     }
+    f16x8 hi[CT][4], lo[CT][4];
+    f32x4 back[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const size_t at = size_t(min(tok0 / 16 + c, last_tile)) * blocks + b;
       const unsigned char* parts = x.parts + at * kPartBytes + lane * 16;
-      f16x8 hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        hi[j] = *reinterpret_cast<const f16x8*>(parts + j * 1024);
-        lo[j] = *reinterpret_cast<const f16x8*>(parts + 4096 + j * 1024);
+        hi[c][j] = *reinterpret_cast<const f16x8*>(parts + j * 1024);
+        lo[c][j] = *reinterpret_cast<const f16x8*>(parts + 4096 + j * 1024);
       }
-      const f32x4 back = *reinterpret_cast<const f32x4*>(x.back + at * 16 + 4 * g);
-#pragma unroll
-      for (int n = 0; n < NA; ++n)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int p = j * kPer / 4;
-            const f16x8 wq = unpack8(wb[n].q[i][j], wb[n].z[i][p]);
-            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[j], wq, part, 0, 0, 0);
-            part = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[j], wq, part, 0, 0, 0);
-            if ((j + 1) % (4 / kPer) == 0) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                acc[n][i][c][e] = __builtin_fmaf(part[e], wb[n].s[i][p] * back[e], acc[n][i][c][e]);
-              part = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-          }
-        }
+      back[c] = *reinterpret_cast<const f32x4*>(x.back + at * 16 + 4 * g);
     }
+#pragma unroll
+    for (int n = 0; n < NA; ++n)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const Q4Tile<GROUP, S32> t(wb[n], i, w[0].bf16);
+        f16x8 wq[4];
+        t.unpack(wq);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) t.multiply(wq, hi[c], lo[c], back[c], acc[n][i][c]);
+      }
   }
   f32x4* sums = reinterpret_cast<f32x4*>(dyn);
 #pragma unroll
@@ -426,9 +574,9 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
     f32x4 v[NA];
 #pragma unroll
     for (int n = 0; n < NA; ++n) {
-      v[n] = sums[(n * RT * CT + t) * 64 + lane];
+      v[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int sl = 1; sl < kSlots; ++sl) v[n] += sums[(sl * NT + n * RT * CT + t) * 64 + lane];
+      for (int sl = 0; sl < kSlots; ++sl) v[n] += sums[(sl * NT + n * RT * CT + t) * 64 + lane];
     }
     const int at = row0 + 16 * (t / CT) + r, tok1 = tok0 + 16 * (t % CT) + 4 * g;
     if (at >= rows) continue;
@@ -446,13 +594,13 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
 // waves, one to a SIMD. The tokens' parts of a block reach LDS by DMA (64 KB, two stages, the next under
 // way while a block is multiplied); the weights go from memory to registers, where a wave unpacks them
 // once for its 64 tokens. All blocks are walked in turn, the slots' sums folded at their ends.
-template <bool GATE, int GROUP>
+template <bool GATE, int GROUP, bool S32>
 __global__ void __launch_bounds__(256, 1)
 q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
                 int row_tiles, int tok_tiles) {
   constexpr int NA = GATE ? 2 : 1, RT = 4, CT = 4, RM = RT / NA;  // RM: row tiles per matrix
   constexpr int kPer = kBlock / GROUP;
-  constexpr int kStage = 8 * kPartBytes;
+  constexpr int kBacks = 8 * 16 * 4, kStage = 8 * kPartBytes + kBacks;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -460,28 +608,27 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   int row_tile, tok_tile;
   tile_of_block<GATE>(blockIdx.x, row_tiles, tok_tiles, row_tile, tok_tile);
   const int row0 = (row_tile * 2 + wm) * 16 * RM, tok0 = tok_tile * 128;
-  const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
+  const int blocks = (cols + kBlock - 1) / kBlock;
   const int last_tile = (T - 1) / 16;
-  int row[RM];
-#pragma unroll
-  for (int i = 0; i < RM; ++i) row[i] = min(row0 + 16 * i + r, rows - 1);
-  const Q4View w[2] = {w0, w1};
+  const Q4Rows<RM, GROUP, S32> w[2] = {{w0, scale_type, row0, rows, cols, r},
+                                       {GATE ? w1 : w0, scale_type, row0, rows, cols, r}};
+  const bool bf16 = w[0].bf16;
   const unsigned base = lds_address(dyn);
-  // Wave i brings token tiles 2i and 2i + 1 of a block: 16 transfers of 1 KB.
+  // Wave i brings token tiles 2i and 2i + 1 of a block: 16 transfers of 1 KB, and half a one of powers.
+  const unsigned char* from[2];
+  const float* from_back;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    from[c] = x.parts + size_t(min(tok_tile * 8 + 2 * wave + c, last_tile)) * blocks * kPartBytes;
+  from_back = x.back + size_t(min(tok_tile * 8 + int(threadIdx.x) / 16 % 8, last_tile)) * blocks * 16 + r;
   auto stage = [&](int b, int s) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const size_t at = size_t(min(tok_tile * 8 + 2 * wave + c, last_tile)) * blocks + b;
-      const unsigned char* src = x.parts + at * kPartBytes + lane * 16;
-      const unsigned to = base + s * kStage + (2 * wave + c) * kPartBytes;
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dma16(src + j * 1024, to + j * 1024);
-    }
+      for (int j = 0; j < 8; ++j)
+        dma16_at(from[c] + size_t(b) * kPartBytes + j * 1024, lane * 16,
+                 base + s * kStage + (2 * wave + c) * kPartBytes + j * 1024);
   };
-  size_t tile_at[CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) tile_at[c] = size_t(min(tok_tile * 8 + 4 * wn + c, last_tile)) * blocks;
-
   f32x4 total[RT][CT], acc[RT][CT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -490,14 +637,15 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
       total[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-  Q4Block<RM, GROUP> next[NA];
-  f32x4 next_back[CT];
+  Q4Block<RM, GROUP, S32> next[NA];
+  float next_back = 0.f;
   auto fetch = [&](int b) {
 #pragma unroll
-    for (int n = 0; n < NA; ++n) next[n].load(w[n], scale_type, row, b, g, cols, groups);
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-      next_back[c] = *reinterpret_cast<const f32x4*>(x.back + (tile_at[c] + b) * 16 + 4 * g);
+    for (int n = 0; n < NA; ++n) next[n].load(w[n], b, g);
+    next_back = from_back[size_t(b) * 16];
+  };
+  auto put_back = [&](int s) {
+    if (threadIdx.x < 128) reinterpret_cast<float*>(dyn + s * kStage + 8 * kPartBytes)[threadIdx.x] = next_back;
   };
   stage(0, 0);
   fetch(0);
@@ -505,25 +653,22 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   for (int slot = 0; slot < kSlots; ++slot) {
     const int b1 = slot_block(slot + 1, blocks);
     for (; b < b1; ++b) {
+      put_back(b & 1);
       wait_vmcnt<0>();
       __syncthreads();
-      Q4Block<RM, GROUP> wb[NA];
-      f32x4 back[CT];
+      Q4Block<RM, GROUP, S32> wb[NA];
 #pragma unroll
       for (int n = 0; n < NA; ++n) wb[n] = next[n];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) back[c] = next_back[c];
       if (b + 1 < blocks) {
         fetch(b + 1);
         stage(b + 1, (b + 1) & 1);
       }
-      if constexpr (GROUP != 128) {
-#pragma unroll
-        for (int n = 0; n < NA; ++n)
-#pragma unroll
-          for (int i = 0; i < RM; ++i) transpose4(wb[n].q[i]);
-      }
+      using Tile = Q4Tile<GROUP, S32>;
+      const Tile t[RT] = {Tile(wb[0], 0, bf16), Tile(wb[0], 1, bf16),
+                          GATE ? Tile(wb[NA - 1], 0, bf16) : Tile(wb[0], RM - 2, bf16),
+                          Tile(wb[NA - 1], RM - 1, bf16)};
       const unsigned char* parts = dyn + (b & 1) * kStage + 4 * wn * kPartBytes + lane * 16;
+      const float* backs = reinterpret_cast<const float*>(dyn + (b & 1) * kStage + 8 * kPartBytes) + 64 * wn + 4 * g;
       f32x4 part[RT][CT];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -536,8 +681,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-          const Q4Block<RM, GROUP>& wi = wb[i / RM];
-          const f16x8 wq = unpack8(wi.q[i % RM][j], wi.z[i % RM][p]);
+          const f16x8 wq = t[i].weights(j);
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             if (j % (4 / kPer) == 0) part[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -546,13 +690,18 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
 #pragma unroll
           for (int c = 0; c < CT; ++c)
             part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[c], wq, part[i][c], 0, 0, 0);
-          if ((j + 1) % (4 / kPer) == 0) {
-            const float s = wi.s[i % RM][p];
+        }
+        if ((j + 1) % (4 / kPer) == 0) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+          for (int c = 0; c < CT; ++c) {
+            const f32x4 back = *reinterpret_cast<const f32x4*>(backs + 16 * c);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+              const float sc = t[i].scale[p];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                acc[i][c][e] = __builtin_fmaf(part[i][c][e], s * back[c][e], acc[i][c][e]);
+                acc[i][c][e] = __builtin_fmaf(part[i][c][e], sc * back[e], acc[i][c][e]);
+            }
           }
         }
       }
@@ -561,7 +710,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        total[i][c] = slot == 0 ? acc[i][c] : total[i][c] + acc[i][c];
+        total[i][c] += acc[i][c];
         acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
@@ -587,8 +736,8 @@ int check_matrix_q4(const ie_matrix_q4& m, const char* who) {
     return fail(IE_HIP_EINVAL, std::string(who) + ": empty weight matrix");
   if (m.group != 32 && m.group != 64 && m.group != 128)
     return fail(IE_HIP_EINVAL, std::string(who) + ": groups must be of 32, 64 or 128 columns");
-  if (m.cols % 32)
-    return fail(IE_HIP_EINVAL, std::string(who) + ": cols must be a multiple of 32");
+  if (m.cols % 32 || m.cols > kMaxCols)
+    return fail(IE_HIP_EINVAL, std::string(who) + ": cols must be a multiple of 32 up to 16,777,216");
   if (m.scale_dtype != IE_KV_F32 && m.scale_dtype != IE_KV_F16 && m.scale_dtype != IE_KV_BF16)
     return fail(IE_HIP_EINVAL, std::string(who) + ": unknown scale_dtype " + std::to_string(m.scale_dtype));
   if (reinterpret_cast<uintptr_t>(m.data) & 15)
@@ -598,8 +747,16 @@ int check_matrix_q4(const ie_matrix_q4& m, const char* who) {
   return IE_HIP_OK;
 }
 
-// Tokens that a launch splits by itself; more are split once into the workspace.
-constexpr int kFewTokens = 16;
+constexpr int kFewLds = 160 * 1024;
+
+// Whether the activations are split once into the workspace, by a launch of their own: more than 16
+// tokens, or more than q4_few_kernel holds in LDS beside its stages (57 KB of parts up to 1,024 columns,
+// whose stages are the smaller, 45 KB above).
+bool needs_parts(int T, int cols) {
+  const int64_t places = T == 1 ? 1 : T <= 4 ? 4 : 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
+  return T > 16 || places * blocks > (blocks <= kSlots ? 112 : 88);
+}
+
 
 struct Q4Launch {
   Q4Out out;
@@ -611,22 +768,41 @@ struct Q4Launch {
   const char* who;
 
   int too_many() const { return fail(IE_HIP_EINVAL, std::string(who) + ": too many rows or tokens"); }
-  template <bool GATE, int RT, int GROUP>
-  int few() const {
-    const int64_t row_groups = (int64_t(rows) + 16 * RT - 1) / (16 * RT);
-    if (row_groups * 64 * kSlots > int64_t(UINT32_MAX)) return too_many();
-    hipLaunchKernelGGL((q4_few_kernel<GATE, RT, GROUP>), dim3(unsigned(row_groups)), dim3(64 * kSlots), 0,
-                       stream, out, x, w0, w1, scale_type, T, rows, cols, int(row_groups));
-    return IE_HIP_OK;
+  template <class Kernel>
+  int more_lds(Kernel kernel, int bytes) const {
+    return check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                     "hipFuncSetAttribute(q4)");
   }
-  template <bool GATE, int RT, int CT, int GROUP>
+  // False where the tokens' parts do not fit.
+  template <bool GATE, int GROUP, bool S32, int TP, int SB, bool SPLIT>
+  bool few_go(int64_t row_tiles, int64_t cus, int* rc) const {
+    using F = FewShape<GATE, GROUP, TP, SB, SPLIT>;
+    const int64_t lds = F::bytes((int64_t(cols) + kBlock - 1) / kBlock);
+    if (lds > kFewLds) return false;
+    const auto kernel = q4_few_kernel<GATE, GROUP, S32, TP, SB, SPLIT>;
+    static const int more = more_lds(kernel, kFewLds);
+    if ((*rc = more)) return true;
+    const int64_t each = std::min<int64_t>(2, kFewLds / lds);  // workgroups of a compute unit
+    const int64_t grid = std::min(SPLIT ? row_tiles : (row_tiles + kSlots - 1) / kSlots, each * cus);
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(64 * kSlots), unsigned(lds), stream, out, x, w0,
+                       w1, scale_type, T, rows, cols, int(row_tiles));
+    return true;
+  }
+  template <bool GATE, int GROUP, bool S32, int TP>
+  bool few(int64_t row_tiles, int64_t cus, int* rc) const {
+    constexpr int kMost = GATE ? 2 : 4;
+    if (row_tiles >= 8 * cus) return few_go<GATE, GROUP, S32, TP, kMost, false>(row_tiles, cus, rc);
+    return cols <= kSlots * kBlock ? few_go<GATE, GROUP, S32, TP, 1, true>(row_tiles, cus, rc)
+                                   : few_go<GATE, GROUP, S32, TP, kMost, true>(row_tiles, cus, rc);
+  }
+  template <bool GATE, int RT, int CT, int GROUP, bool S32>
   int slots() const {
     constexpr int kLds = kSlots * (GATE ? 2 : 1) * RT * CT * 1024;
-    const auto kernel = q4_slots_kernel<GATE, RT, CT, GROUP>;
+    const auto kernel = q4_slots_kernel<GATE, RT, CT, GROUP, S32>;
     if (kLds > 64 * 1024) {
-      static const hipError_t attr = hipFuncSetAttribute(
-          reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-      if (int rc = check_hip(attr, "hipFuncSetAttribute(q4)")) return rc;
+      static const int rc = more_lds(kernel, kLds);
+      if (rc) return rc;
     }
     const int64_t row_groups = (int64_t(rows) + 16 * RT - 1) / (16 * RT);
     const int64_t grid = row_groups * ((int64_t(T) + 16 * CT - 1) / (16 * CT));
@@ -635,38 +811,44 @@ struct Q4Launch {
                        scale_type, T, rows, cols, int(row_groups));
     return IE_HIP_OK;
   }
-  template <bool GATE, int GROUP>
+  template <bool GATE, int GROUP, bool S32>
   int tiles() const {
-    constexpr int kLds = 2 * 8 * kPartBytes, kRows = GATE ? 64 : 128;
-    const auto kernel = q4_tiles_kernel<GATE, GROUP>;
-    static const hipError_t attr = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (int rc = check_hip(attr, "hipFuncSetAttribute(q4)")) return rc;
+    constexpr int kLds = 2 * (8 * kPartBytes + 512), kRows = GATE ? 64 : 128;
+    const auto kernel = q4_tiles_kernel<GATE, GROUP, S32>;
+    static const int rc = more_lds(kernel, kLds);
+    if (rc) return rc;
     const int64_t row_tiles = (int64_t(rows) + kRows - 1) / kRows, tok_tiles = (int64_t(T) + 127) / 128;
     if (row_tiles * tok_tiles * 256 > int64_t(UINT32_MAX)) return too_many();
     hipLaunchKernelGGL(kernel, dim3(unsigned(row_tiles * tok_tiles)), dim3(256), kLds, stream, out, parts,
                        w0, w1, scale_type, T, rows, cols, int(row_tiles), int(tok_tiles));
     return IE_HIP_OK;
   }
-  template <bool GATE, int GROUP>
+  template <bool GATE, int GROUP, bool S32>
   int run() const {
     const int64_t row_tiles = (int64_t(rows) + 15) / 16;
     const int64_t cus = device_compute_units();
-    if (T <= kFewTokens) {
-      if (row_tiles >= 8 * cus) return few<GATE, 4, GROUP>();
-      if (row_tiles >= 4 * cus) return few<GATE, 2, GROUP>();
-      return few<GATE, 1, GROUP>();
+    int rc = IE_HIP_OK;
+    if (!needs_parts(T, cols)) {
+      if (T == 1 ? few<GATE, GROUP, S32, 1>(row_tiles, cus, &rc)
+                 : T <= 4 ? few<GATE, GROUP, S32, 4>(row_tiles, cus, &rc)
+                          : few<GATE, GROUP, S32, 16>(row_tiles, cus, &rc))
+        return rc;
+      return fail(IE_HIP_EINVAL, std::string(who) + ": activations past a workgroup's memory");
     }
     const int64_t tok_tiles = (int64_t(T) + 15) / 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
     if (tok_tiles * blocks * 256 > int64_t(UINT32_MAX)) return too_many();
-    hipLaunchKernelGGL(q4_split_kernel<GROUP == 128>, dim3(unsigned(tok_tiles * blocks)), dim3(256), 0,
+    hipLaunchKernelGGL(q4_split_kernel<GROUP == kBlock>, dim3(unsigned(tok_tiles * blocks)), dim3(256), 0,
                        stream, parts, x, T, cols, int(blocks));
     const int64_t big = ((int64_t(rows) + (GATE ? 63 : 127)) / (GATE ? 64 : 128)) * ((int64_t(T) + 127) / 128);
-    if (2 * big >= cus) return tiles<GATE, GROUP>();
-    if (T <= 32) return row_tiles >= 4 * cus ? slots<GATE, 2, 2, GROUP>() : slots<GATE, 1, 2, GROUP>();
+    if (2 * big >= cus) return tiles<GATE, GROUP, S32>();
+    if (T <= 32) return row_tiles >= 4 * cus ? slots<GATE, 2, 2, GROUP, S32>() : slots<GATE, 1, 2, GROUP, S32>();
     if constexpr (!GATE)
-      if (row_tiles >= 2 * cus) return slots<GATE, 2, 4, GROUP>();
-    return slots<GATE, 1, 4, GROUP>();
+      if (row_tiles >= 2 * cus) return slots<GATE, 2, 4, GROUP, S32>();
+    return slots<GATE, 1, 4, GROUP, S32>();
+  }
+  template <bool GATE, int GROUP>
+  int run() const {
+    return scale_type == IE_KV_F32 ? run<GATE, GROUP, true>() : run<GATE, GROUP, false>();
   }
   template <bool GATE>
   int run(int group) const {
@@ -678,6 +860,11 @@ Parts parts_of(void* workspace, int T, int cols) {
   unsigned char* base = static_cast<unsigned char*>(workspace);
   const size_t n = part_tiles(T) * ((size_t(cols) + kBlock - 1) / kBlock);
   return Parts{base, reinterpret_cast<float*>(base + n * kPartBytes)};
+}
+
+Q4View view_of(const ie_matrix_q4& w) {
+  return Q4View{static_cast<const uint8_t*>(w.data), static_cast<const uint8_t*>(w.scale),
+                static_cast<const uint8_t*>(w.zero)};
 }
 
 int launch_q4(bool gate, float* y, const float* x, const ie_matrix_q4& w, const ie_matrix_q4* w2,
@@ -704,11 +891,8 @@ int launch_q4(bool gate, float* y, const float* x, const ie_matrix_q4& w, const 
     return fail(IE_HIP_EINVAL, std::string(who) + ": the workspace must be 16-byte aligned");
   const Q4Launch launch{Q4Out{y, bias, accumulate, split},
                         x,
-                        Q4View{static_cast<const uint8_t*>(w.data), w.scale,
-                               static_cast<const uint8_t*>(w.zero)},
-                        w2 ? Q4View{static_cast<const uint8_t*>(w2->data), w2->scale,
-                                    static_cast<const uint8_t*>(w2->zero)}
-                           : Q4View{nullptr, nullptr, nullptr},
+                        view_of(w),
+                        w2 ? view_of(*w2) : Q4View{nullptr, nullptr, nullptr},
                         w.scale_dtype,
                         T,
                         w.rows,
@@ -726,7 +910,7 @@ int launch_q4(bool gate, float* y, const float* x, const ie_matrix_q4& w, const 
 using namespace iehip;
 
 extern "C" size_t ie_hip_matmul_q4_workspace_bytes(int T, int cols) {
-  if (T <= kFewTokens || cols <= 0) return 0;
+  if (T <= 0 || cols <= 0 || !needs_parts(T, cols)) return 0;
   return part_tiles(T) * ((size_t(cols) + kBlock - 1) / kBlock) * (kPartBytes + 64);
 }
 
