@@ -590,21 +590,22 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   }
 }
 
-// Prompts: 128 rows (64 of each matrix with GATE) x 128 tokens a workgroup, a wave 64 x 64 of them: 2 x 2
-// waves, one to a SIMD. The tokens' parts of a block reach LDS by DMA (64 KB, two stages, the next under
+// Prompts: 128 rows (64 of each matrix with GATE) x 128 tokens a workgroup, a wave 64 x 32 of them: 2 x 4
+// waves, two to a SIMD, so that one's VALU work stands beside the other's products (4 waves of 64 x 64,
+// which unpack half as often: 4,096 x 4,096 at 2,048 tokens 258 us). The tokens' parts of a block reach LDS by DMA (64 KB, two stages, the next under
 // way while a block is multiplied); the weights go from memory to registers, where a wave unpacks them
-// once for its 64 tokens. All blocks are walked in turn, the slots' sums folded at their ends.
+// once for its 32 tokens. All blocks are walked in turn, the slots' sums folded at their ends.
 template <bool GATE, int GROUP, bool S32>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(512)
 q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
                 int row_tiles, int tok_tiles) {
-  constexpr int NA = GATE ? 2 : 1, RT = 4, CT = 4, RM = RT / NA;  // RM: row tiles per matrix
+  constexpr int NA = GATE ? 2 : 1, RT = 4, CT = 2, RM = RT / NA;  // RM: row tiles per matrix
   constexpr int kPer = kBlock / GROUP;
   constexpr int kBacks = 8 * 16 * 4, kStage = 8 * kPartBytes + kBacks;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, r = lane & 15, wm = wave >> 1, wn = wave & 1;
+  const int g = lane >> 4, r = lane & 15, wm = wave >> 2, wn = wave & 3;
   int row_tile, tok_tile;
   tile_of_block<GATE>(blockIdx.x, row_tiles, tok_tiles, row_tile, tok_tile);
   const int row0 = (row_tile * 2 + wm) * 16 * RM, tok0 = tok_tile * 128;
@@ -614,20 +615,14 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
                                        {GATE ? w1 : w0, scale_type, row0, rows, cols, r}};
   const bool bf16 = w[0].bf16;
   const unsigned base = lds_address(dyn);
-  // Wave i brings token tiles 2i and 2i + 1 of a block: 16 transfers of 1 KB, and half a one of powers.
-  const unsigned char* from[2];
-  const float* from_back;
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-    from[c] = x.parts + size_t(min(tok_tile * 8 + 2 * wave + c, last_tile)) * blocks * kPartBytes;
-  from_back = x.back + size_t(min(tok_tile * 8 + int(threadIdx.x) / 16 % 8, last_tile)) * blocks * 16 + r;
+  // Wave i brings token tile i of a block, 8 transfers of 1 KB; the first two waves the powers.
+  const unsigned char* from = x.parts + size_t(min(tok_tile * 8 + wave, last_tile)) * blocks * kPartBytes;
+  const float* from_back = x.back + size_t(min(tok_tile * 8 + int(threadIdx.x) / 16 % 8, last_tile)) * blocks * 16 + r;
   auto stage = [&](int b, int s) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        dma16_at(from[c] + size_t(b) * kPartBytes + j * 1024, lane * 16,
-                 base + s * kStage + (2 * wave + c) * kPartBytes + j * 1024);
+    for (int j = 0; j < 8; ++j)
+      dma16_at(from + size_t(b) * kPartBytes + j * 1024, lane * 16,
+               base + s * kStage + wave * kPartBytes + j * 1024);
   };
   f32x4 total[RT][CT], acc[RT][CT];
 #pragma unroll
@@ -667,8 +662,8 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
       const Tile t[RT] = {Tile(wb[0], 0, bf16), Tile(wb[0], 1, bf16),
                           GATE ? Tile(wb[NA - 1], 0, bf16) : Tile(wb[0], RM - 2, bf16),
                           Tile(wb[NA - 1], RM - 1, bf16)};
-      const unsigned char* parts = dyn + (b & 1) * kStage + 4 * wn * kPartBytes + lane * 16;
-      const float* backs = reinterpret_cast<const float*>(dyn + (b & 1) * kStage + 8 * kPartBytes) + 64 * wn + 4 * g;
+      const unsigned char* parts = dyn + (b & 1) * kStage + 2 * wn * kPartBytes + lane * 16;
+      const float* backs = reinterpret_cast<const float*>(dyn + (b & 1) * kStage + 8 * kPartBytes) + 32 * wn + 4 * g;
       f32x4 part[RT][CT];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -722,7 +717,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int tok = tok0 + (4 * wn + c) * 16 + 4 * g + e;
+        const int tok = tok0 + (2 * wn + c) * 16 + 4 * g + e;
         if (tok >= T) continue;
         float o = total[i][c][e];
         if constexpr (GATE) o = silu(o) * total[RM + i][c][e];
@@ -818,8 +813,8 @@ struct Q4Launch {
     static const int rc = more_lds(kernel, kLds);
     if (rc) return rc;
     const int64_t row_tiles = (int64_t(rows) + kRows - 1) / kRows, tok_tiles = (int64_t(T) + 127) / 128;
-    if (row_tiles * tok_tiles * 256 > int64_t(UINT32_MAX)) return too_many();
-    hipLaunchKernelGGL(kernel, dim3(unsigned(row_tiles * tok_tiles)), dim3(256), kLds, stream, out, parts,
+    if (row_tiles * tok_tiles * 512 > int64_t(UINT32_MAX)) return too_many();
+    hipLaunchKernelGGL(kernel, dim3(unsigned(row_tiles * tok_tiles)), dim3(512), kLds, stream, out, parts,
                        w0, w1, scale_type, T, rows, cols, int(row_tiles), int(tok_tiles));
     return IE_HIP_OK;
   }
