@@ -590,18 +590,22 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   }
 }
 
+// A stage of q4_tiles_kernel in LDS: the parts of 8 token tiles, their powers, 8 row tiles' weights with
+// their scales and zero points.
+constexpr int kTileBacks = 8 * kPartBytes, kTileWeights = kTileBacks + 8 * 256, kTileUnit = 1024 + 512;
+constexpr int kTileStage = kTileWeights + 8 * kTileUnit;
+
 // Prompts: 128 rows (64 of each matrix with GATE) x 128 tokens a workgroup, a wave 64 x 32 of them: 2 x 4
 // waves, two to a SIMD, so that one's VALU work stands beside the other's products (4 waves of 64 x 64,
-// which unpack half as often: 4,096 x 4,096 at 2,048 tokens 258 us). The tokens' parts of a block reach LDS by DMA (64 KB, two stages, the next under
-// way while a block is multiplied); the weights go from memory to registers, where a wave unpacks them
-// once for its 32 tokens. All blocks are walked in turn, the slots' sums folded at their ends.
+// which unpack half as often, one to a SIMD: 4,096 x 4,096 at 2,048 tokens 258 us). A block's parts and
+// weights reach LDS by DMA (73 KB, two stages, the next under way while a block is multiplied). All blocks
+// are walked in turn, the slots' sums folded at their ends.
 template <bool GATE, int GROUP, bool S32>
 __global__ void __launch_bounds__(512)
 q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
                 int row_tiles, int tok_tiles) {
   constexpr int NA = GATE ? 2 : 1, RT = 4, CT = 2, RM = RT / NA;  // RM: row tiles per matrix
-  constexpr int kPer = kBlock / GROUP;
-  constexpr int kBacks = 8 * 16 * 4, kStage = 8 * kPartBytes + kBacks;
+  constexpr int kPer = kBlock / GROUP, kSize = S32 ? 4 : 2;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -609,20 +613,34 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   int row_tile, tok_tile;
   tile_of_block<GATE>(blockIdx.x, row_tiles, tok_tiles, row_tile, tok_tile);
   const int row0 = (row_tile * 2 + wm) * 16 * RM, tok0 = tok_tile * 128;
-  const int blocks = (cols + kBlock - 1) / kBlock;
+  const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
   const int last_tile = (T - 1) / 16;
-  const Q4Rows<RM, GROUP, S32> w[2] = {{w0, scale_type, row0, rows, cols, r},
-                                       {GATE ? w1 : w0, scale_type, row0, rows, cols, r}};
-  const bool bf16 = w[0].bf16;
+  const bool bf16 = scale_type == IE_KV_BF16;
   const unsigned base = lds_address(dyn);
-  // Wave i brings token tile i of a block, 8 transfers of 1 KB; the first two waves the powers.
-  const unsigned char* from = x.parts + size_t(min(tok_tile * 8 + wave, last_tile)) * blocks * kPartBytes;
-  const float* from_back = x.back + size_t(min(tok_tile * 8 + int(threadIdx.x) / 16 % 8, last_tile)) * blocks * 16 + r;
-  auto stage = [&](int b, int s) {
+  // Wave i brings token tile i of a block (8 transfers of 1 KB, one of powers) and row tile i of the
+  // workgroup's 8 (one each of weights, scales and zero points); waves 4 wm .. 4 wm + 3 use the latter.
+  const size_t part_at = size_t(min(tok_tile * 8 + wave, last_tile)) * blocks;
+  const Q4View& w = GATE && wave % 4 >= RM ? w1 : w0;
+  const int load_row = min((row_tile * 2 + wm) * 16 * RM + wave % RM * 16, rows - 1);
+  const int last_row = rows - 1 - load_row;
+  const uint8_t* data = w.data + size_t(load_row) * (cols / 2);
+  const uint8_t* scale = w.scale + size_t(load_row) * groups * kSize;
+  const uint8_t* zero = w.zero ? w.zero + size_t(load_row) * groups : kEight;
+  const uint32_t zero_step = w.zero ? 1 : 0;
+  const uint32_t data_row = uint32_t(min(lane / 4, last_row)) * (cols / 2);
+  const uint32_t scale_row = uint32_t(min(r, last_row)) * groups;
+  auto issue = [&](int b, int s) {
+    const unsigned to = base + s * kTileStage;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      dma16_at(from + size_t(b) * kPartBytes + j * 1024, lane * 16,
-               base + s * kStage + wave * kPartBytes + j * 1024);
+      dma16_at(x.parts + (part_at + b) * kPartBytes + j * 1024, lane * 16, to + wave * kPartBytes + j * 1024);
+    dma_word<4>(x.back + (part_at + b) * 16, r * 4, to + kTileBacks + wave * 256);
+    const int word = min(4 * b + ((lane & 3) ^ (lane >> 4)), cols / 32 - 1);
+    const unsigned unit = to + kTileWeights + wave * kTileUnit;
+    dma16_at(data, data_row + word * 16, unit);
+    const uint32_t at = scale_row + min(b * kPer + g * kPer / 4, groups - 1);
+    dma_word<kSize>(scale, at * kSize, unit + 1024);
+    dma_word<1>(zero, at * zero_step, unit + 1280);
   };
   f32x4 total[RT][CT], acc[RT][CT];
 #pragma unroll
@@ -632,71 +650,66 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
       total[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-  Q4Block<RM, GROUP, S32> next[NA];
-  float next_back = 0.f;
-  auto fetch = [&](int b) {
-#pragma unroll
-    for (int n = 0; n < NA; ++n) next[n].load(w[n], b, g);
-    next_back = from_back[size_t(b) * 16];
-  };
-  auto put_back = [&](int s) {
-    if (threadIdx.x < 128) reinterpret_cast<float*>(dyn + s * kStage + 8 * kPartBytes)[threadIdx.x] = next_back;
-  };
-  stage(0, 0);
-  fetch(0);
+  issue(0, 0);
   int b = 0;
   for (int slot = 0; slot < kSlots; ++slot) {
     const int b1 = slot_block(slot + 1, blocks);
     for (; b < b1; ++b) {
-      put_back(b & 1);
-      wait_vmcnt<0>();
-      __syncthreads();
-      Q4Block<RM, GROUP, S32> wb[NA];
+      // This wave's transfers have landed, then everyone's, and the other stage has been read.
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (b + 1 < blocks) issue(b + 1, (b + 1) & 1);
+      const unsigned char* from = dyn + (b & 1) * kTileStage;
+      const unsigned char* parts = from + 2 * wn * kPartBytes + lane * 16;
+      f16x8 hi[2][CT], lo[2][CT];
+      auto read = [&](int j) {
 #pragma unroll
-      for (int n = 0; n < NA; ++n) wb[n] = next[n];
-      if (b + 1 < blocks) {
-        fetch(b + 1);
-        stage(b + 1, (b + 1) & 1);
-      }
+        for (int c = 0; c < CT; ++c) {
+          hi[j & 1][c] = *reinterpret_cast<const f16x8*>(parts + c * kPartBytes + j * 1024);
+          lo[j & 1][c] = *reinterpret_cast<const f16x8*>(parts + c * kPartBytes + 4096 + j * 1024);
+        }
+      };
+      read(0);
       using Tile = Q4Tile<GROUP, S32>;
-      const Tile t[RT] = {Tile(wb[0], 0, bf16), Tile(wb[0], 1, bf16),
-                          GATE ? Tile(wb[NA - 1], 0, bf16) : Tile(wb[0], RM - 2, bf16),
-                          Tile(wb[NA - 1], RM - 1, bf16)};
-      const unsigned char* parts = dyn + (b & 1) * kStage + 2 * wn * kPartBytes + lane * 16;
-      const float* backs = reinterpret_cast<const float*>(dyn + (b & 1) * kStage + 8 * kPartBytes) + 32 * wn + 4 * g;
+      auto tile = [&](int i) {
+        const unsigned char* unit = from + kTileWeights + (4 * wm + i) * kTileUnit;
+        const u32x4 q = *reinterpret_cast<const u32x4*>(unit + (r * 4 + (g ^ (r >> 2))) * 16);
+        uint32_t sc[kPer], ze[kPer];
+#pragma unroll
+        for (int p = 0; p < kPer; ++p) {
+          sc[p] = reinterpret_cast<const uint32_t*>(unit + 1024)[p * 4 / kPer * 16 + r];
+          if constexpr (!S32) sc[p] &= 0xFFFFu;
+          ze[p] = reinterpret_cast<const uint32_t*>(unit + 1280)[p * 4 / kPer * 16 + r] & 0xFFu;
+        }
+        return Tile(q, sc, ze, bf16);
+      };
+      const Tile t[RT] = {tile(0), tile(1), tile(2), tile(3)};
       f32x4 part[RT][CT];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int p = j * kPer / 4;
-        f16x8 hi[CT], lo[CT];
+        if (j < 3) read(j + 1);
+        f16x8 wq[RT];
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          hi[c] = *reinterpret_cast<const f16x8*>(parts + c * kPartBytes + j * 1024);
-          lo[c] = *reinterpret_cast<const f16x8*>(parts + c * kPartBytes + 4096 + j * 1024);
-        }
+        for (int i = 0; i < RT; ++i) wq[i] = t[i].weights(j);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          const f16x8 wq = t[i].weights(j);
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            if (j % (4 / kPer) == 0) part[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-            part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[c], wq, part[i][c], 0, 0, 0);
-          }
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int c = 0; c < CT; ++c)
-            part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[c], wq, part[i][c], 0, 0, 0);
-        }
+            part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                hi[j & 1][c], wq[i], j % (4 / kPer) == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : part[i][c], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+            part[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[j & 1][c], wq[i], part[i][c], 0, 0, 0);
         if ((j + 1) % (4 / kPer) == 0) {
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
-            const f32x4 back = *reinterpret_cast<const f32x4*>(backs + 16 * c);
+            const f32x4 back = *reinterpret_cast<const f32x4*>(from + kTileBacks + (2 * wn + c) * 256 + 16 * g);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              const float sc = t[i].scale[p];
+            for (int i = 0; i < RT; ++i)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                acc[i][c][e] = __builtin_fmaf(part[i][c][e], sc * back[e], acc[i][c][e]);
-            }
+                acc[i][c][e] = __builtin_fmaf(part[i][c][e], t[i].scale[j * kPer / 4] * back[e], acc[i][c][e]);
           }
         }
       }
@@ -808,7 +821,7 @@ struct Q4Launch {
   }
   template <bool GATE, int GROUP, bool S32>
   int tiles() const {
-    constexpr int kLds = 2 * (8 * kPartBytes + 512), kRows = GATE ? 64 : 128;
+    constexpr int kLds = 2 * kTileStage, kRows = GATE ? 64 : 128;
     const auto kernel = q4_tiles_kernel<GATE, GROUP, S32>;
     static const int rc = more_lds(kernel, kLds);
     if (rc) return rc;
