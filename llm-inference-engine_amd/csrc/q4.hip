@@ -629,11 +629,13 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   const uint32_t zero_step = w.zero ? 1 : 0;
   const uint32_t data_row = uint32_t(min(lane / 4, last_row)) * (cols / 2);
   const uint32_t scale_row = uint32_t(min(r, last_row)) * groups;
-  auto issue = [&](int b, int s) {
+  // In four parts, so that a block's products start before all of the next one's transfers are taken.
+  auto issue = [&](int b, int s, int part) {
     const unsigned to = base + s * kTileStage;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 2 * part; j < 2 * part + 2; ++j)
       dma16_at(x.parts + (part_at + b) * kPartBytes + j * 1024, lane * 16, to + wave * kPartBytes + j * 1024);
+    if (part > 0) return;
     dma_word<4>(x.back + (part_at + b) * 16, r * 4, to + kTileBacks + wave * 256);
     const int word = min(4 * b + ((lane & 3) ^ (lane >> 4)), cols / 32 - 1);
     const unsigned unit = to + kTileWeights + wave * kTileUnit;
@@ -650,14 +652,14 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
       total[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
       acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-  issue(0, 0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) issue(0, 0, j);
   int b = 0;
   for (int slot = 0; slot < kSlots; ++slot) {
     const int b1 = slot_block(slot + 1, blocks);
     for (; b < b1; ++b) {
       // This wave's transfers have landed, then everyone's, and the other stage has been read.
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (b + 1 < blocks) issue(b + 1, (b + 1) & 1);
       const unsigned char* from = dyn + (b & 1) * kTileStage;
       const unsigned char* parts = from + 2 * wn * kPartBytes + lane * 16;
       f16x8 hi[2][CT], lo[2][CT];
@@ -687,6 +689,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (j < 3) read(j + 1);
+        if (b + 1 < blocks) issue(b + 1, (b + 1) & 1, j);
         f16x8 wq[RT];
 #pragma unroll
         for (int i = 0; i < RT; ++i) wq[i] = t[i].weights(j);
