@@ -239,8 +239,9 @@ struct Q4Tile {
     for (int j = 0; j < 4; ++j) wq[j] = weights(j);
   }
   // The tile times one tile of tokens, added to acc group by group.
-  __device__ __forceinline__ void multiply(const f16x8 (&wq)[4], const f16x8 (&hi)[4], const f16x8 (&lo)[4],
-                                           const f32x4& back, f32x4& acc) const {
+  __device__ __forceinline__ static void multiply(const f16x8 (&wq)[4], const float (&scale)[kPer],
+                                                  const f16x8 (&hi)[4], const f16x8 (&lo)[4],
+                                                  const f32x4& back, f32x4& acc) {
     f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -431,7 +432,7 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
           const Q4Tile<GROUP, S32> t(q, sc, ze, bf16);
           f16x8 wq[4];
           t.unpack(wq);
-          t.multiply(wq, hi, lo, back, acc[n]);
+          t.multiply(wq, t.scale, hi, lo, back, acc[n]);
         }
         if constexpr (!SPLIT)
           while (slot < kSlots && slot_block(slot + 1, blocks) <= b + sb + 1) {
@@ -499,18 +500,22 @@ q4_split_kernel(Parts out, const float* __restrict__ x, int T, int cols, int blo
   if (k8 == 0) out.back[(tile * blocks + b) * 16 + t] = back;
 }
 
-// A few tiles of tokens: the slots' waves as in q4_few_kernel, each with its own blocks' parts straight
-// from the workspace; CT tiles of 16 tokens share the weights.
+// More tokens than q4_few_kernel's, fewer than fill the chip with q4_tiles_kernel's: wave i takes slot i of
+// RT row tiles (of each matrix) by CT tiles of 16 tokens, the tokens' parts straight from the workspace and
+// held while the row tiles go past them, then the slots are added through LDS. What a launch reads over and
+// over is the parts (once per group of row tiles), so row tiles come before token tiles: q/k/v of 300
+// tokens 1 x 4 tiles 10.1 us, RTxCT us; a workgroup's registers leave room for a second one.
 template <bool GATE, int RT, int CT, int GROUP, bool S32>
-__global__ void __launch_bounds__(64 * kSlots)
+__global__ void __launch_bounds__(64 * kSlots, 4)
 q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
-                int row_groups) {
+                int row_groups, int tok_groups) {
   constexpr int NA = GATE ? 2 : 1, NT = NA * RT * CT;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int tok_group = blockIdx.x / row_groups, row_group = blockIdx.x - tok_group * row_groups;
+  int row_group, tok_group;
+  tile_of_block<true>(blockIdx.x, row_groups, tok_groups, row_group, tok_group);
   const int row0 = row_group * 16 * RT, tok0 = tok_group * 16 * CT;
   const int blocks = (cols + kBlock - 1) / kBlock;
   const int last_tile = (T - 1) / 16;
@@ -524,29 +529,20 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   const Q4Rows<RT, GROUP, S32> w[2] = {{w0, scale_type, row0, rows, cols, r},
                                        {GATE ? w1 : w0, scale_type, row0, rows, cols, r}};
   const int b0 = slot_block(wave, blocks), b1 = slot_block(wave + 1, blocks);
-  Q4Block<RT, GROUP, S32> next[NA];
-  if (b0 < b1) {
-#pragma unroll
-    for (int n = 0; n < NA; ++n) next[n].load(w[n], b0, g);
-  }
   for (int b = b0; b < b1; ++b) {
     Q4Block<RT, GROUP, S32> wb[NA];
 #pragma unroll
-    for (int n = 0; n < NA; ++n) wb[n] = next[n];
-    if (b + 1 < b1) {
-#pragma unroll
-      for (int n = 0; n < NA; ++n) next[n].load(w[n], b + 1, g);
-    }
+    for (int n = 0; n < NA; ++n) wb[n].load(w[n], b, g);
     f16x8 hi[CT][4], lo[CT][4];
     f32x4 back[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const size_t at = size_t(min(tok0 / 16 + c, last_tile)) * blocks + b;
-      const unsigned char* parts = x.parts + at * kPartBytes + lane * 16;
+      const unsigned char* parts = x.parts + at * kPartBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        hi[c][j] = *reinterpret_cast<const f16x8*>(parts + j * 1024);
-        lo[c][j] = *reinterpret_cast<const f16x8*>(parts + 4096 + j * 1024);
+        hi[c][j] = *reinterpret_cast<const f16x8*>(parts + (lane * 16 + j * 1024));
+        lo[c][j] = *reinterpret_cast<const f16x8*>(parts + (lane * 16 + 4096 + j * 1024));
       }
       back[c] = *reinterpret_cast<const f32x4*>(x.back + at * 16 + 4 * g);
     }
@@ -558,7 +554,7 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
         f16x8 wq[4];
         t.unpack(wq);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) t.multiply(wq, hi[c], lo[c], back[c], acc[n][i][c]);
+        for (int c = 0; c < CT; ++c) t.multiply(wq, t.scale, hi[c], lo[c], back[c], acc[n][i][c]);
       }
   }
   f32x4* sums = reinterpret_cast<f32x4*>(dyn);
@@ -570,23 +566,22 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
       for (int c = 0; c < CT; ++c)
         sums[(wave * NT + (n * RT + i) * CT + c) * 64 + lane] = acc[n][i][c];
   __syncthreads();
-  for (int t = wave; t < RT * CT; t += kSlots) {
-    f32x4 v[NA];
+  // 4 RT CT quarter tiles, one value of a lane each.
+  for (int q = wave; q < 4 * RT * CT; q += kSlots) {
+    const int tile = q / 4, e = q % 4;
+    const int at = row0 + 16 * (tile / CT) + r, tok = tok0 + 16 * (tile % CT) + 4 * g + e;
+    float v[NA];
 #pragma unroll
     for (int n = 0; n < NA; ++n) {
-      v[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+      v[n] = 0.f;
 #pragma unroll
-      for (int sl = 0; sl < kSlots; ++sl) v[n] += sums[(sl * NT + n * RT * CT + t) * 64 + lane];
+      for (int sl = 0; sl < kSlots; ++sl)
+        v[n] += reinterpret_cast<const float*>(sums + (sl * NT + n * RT * CT + tile) * 64 + lane)[e];
     }
-    const int at = row0 + 16 * (t / CT) + r, tok1 = tok0 + 16 * (t % CT) + 4 * g;
-    if (at >= rows) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (tok1 + e >= T) break;
-      float o = v[0][e];
-      if constexpr (GATE) o = silu(o) * v[NA - 1][e];
-      q4_store(out, rows, tok1 + e, at, o);
-    }
+    if (at >= rows || tok >= T) continue;
+    float o = v[0];
+    if constexpr (GATE) o = silu(o) * v[NA - 1];
+    q4_store(out, rows, tok, at, o);
   }
 }
 
@@ -810,16 +805,13 @@ struct Q4Launch {
   template <bool GATE, int RT, int CT, int GROUP, bool S32>
   int slots() const {
     constexpr int kLds = kSlots * (GATE ? 2 : 1) * RT * CT * 1024;
-    const auto kernel = q4_slots_kernel<GATE, RT, CT, GROUP, S32>;
-    if (kLds > 64 * 1024) {
-      static const int rc = more_lds(kernel, kLds);
-      if (rc) return rc;
-    }
+    static_assert(kLds <= 64 * 1024, "two workgroups of a compute unit");
     const int64_t row_groups = (int64_t(rows) + 16 * RT - 1) / (16 * RT);
-    const int64_t grid = row_groups * ((int64_t(T) + 16 * CT - 1) / (16 * CT));
-    if (grid * 64 * kSlots > int64_t(UINT32_MAX)) return too_many();
-    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(64 * kSlots), kLds, stream, out, parts, w0, w1,
-                       scale_type, T, rows, cols, int(row_groups));
+    const int64_t tok_groups = (int64_t(T) + 16 * CT - 1) / (16 * CT);
+    if (row_groups * tok_groups * 64 * kSlots > int64_t(UINT32_MAX)) return too_many();
+    hipLaunchKernelGGL((q4_slots_kernel<GATE, RT, CT, GROUP, S32>), dim3(unsigned(row_groups * tok_groups)),
+                       dim3(64 * kSlots), kLds, stream, out, parts, w0, w1, scale_type, T, rows, cols,
+                       int(row_groups), int(tok_groups));
     return IE_HIP_OK;
   }
   template <bool GATE, int GROUP, bool S32>
@@ -852,10 +844,10 @@ struct Q4Launch {
                        stream, parts, x, T, cols, int(blocks));
     const int64_t big = ((int64_t(rows) + (GATE ? 63 : 127)) / (GATE ? 64 : 128)) * ((int64_t(T) + 127) / 128);
     if (2 * big >= cus) return tiles<GATE, GROUP, S32>();
-    if (T <= 32) return row_tiles >= 4 * cus ? slots<GATE, 2, 2, GROUP, S32>() : slots<GATE, 1, 2, GROUP, S32>();
-    if constexpr (!GATE)
-      if (row_tiles >= 2 * cus) return slots<GATE, 2, 4, GROUP, S32>();
-    return slots<GATE, 1, 4, GROUP, S32>();
+    constexpr int kMost = GATE ? 2 : 4;  // row tiles of a workgroup: as many as leave every unit one
+    if ((row_tiles + kMost - 1) / kMost * tok_tiles >= cus) return slots<GATE, kMost, 1, GROUP, S32>();
+    if (!GATE && (row_tiles + 1) / 2 * tok_tiles >= cus) return slots<GATE, 2, 1, GROUP, S32>();
+    return slots<GATE, 1, 1, GROUP, S32>();
   }
   template <bool GATE, int GROUP>
   int run() const {
