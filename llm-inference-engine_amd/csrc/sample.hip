@@ -26,13 +26,13 @@
 namespace iehip {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kEach = 16;                  // logits of a thread
-constexpr int kChunk = kThreads * kEach;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the launches over rows
+constexpr int kChunkThreads = 512, kEach = 16;           // of those over chunks, and logits of a thread
+constexpr int kChunk = kChunkThreads * kEach;
 constexpr int kPlaces = 1024;              // bins of the rows' histograms, a thread each
 constexpr int kList = 4096;                // border tokens of a row
 constexpr int kDigits = 2048;
-constexpr int kMaxTokens = 1 << 22;
+constexpr int kMaxTokens = 1 << 22, kMaxChunks = kMaxTokens / kChunk;
 typedef unsigned long long u64;
 
 // Bits of the largest weight, so that n of them stay under 2^63.
@@ -173,9 +173,9 @@ __device__ __forceinline__ int bin_below(double top_place, double at) {
 
 __device__ __forceinline__ float read_logit(float v) { return v == v ? v : -INFINITY; }
 
-// A thread's logits of a chunk: element e of vec4 u is number (u * kThreads + tid) * 4 + e of the chunk.
+// A thread's logits of a chunk: element e of vec4 u is number (u * kChunkThreads + tid) * 4 + e.
 __device__ __forceinline__ int chunk_index(int j) {
-  return ((j >> 2) * kThreads + int(threadIdx.x)) * 4 + (j & 3);
+  return ((j >> 2) * kChunkThreads + int(threadIdx.x)) * 4 + (j & 3);
 }
 __device__ __forceinline__ void load_chunk(float (&v)[kEach], const float* l, int len, bool vec) {
 #pragma unroll
@@ -203,15 +203,16 @@ __device__ __forceinline__ bool beats(float v, int i, float best, int at) {
   return v > best || (v == best && i < at);
 }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kChunkThreads)
 sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
                      double one, int vec) {
+  constexpr int kParts = kChunkThreads / 64;
   __shared__ uint32_t count[kPlaces];
   __shared__ u64 mass[kPlaces];
   __shared__ double powers[64];
-  __shared__ float red_v[kWaves];
-  __shared__ int red_i[kWaves];
-  __shared__ u64 red_m[kWaves];
+  __shared__ float red_v[kParts];
+  __shared__ int red_i[kParts];
+  __shared__ u64 red_m[kParts];
   __shared__ uint32_t far_count;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -220,8 +221,7 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   load_chunk(v, logits + size_t(row) * n + base, len, vec);
   const Row r(s, row, n, one);
   const bool bins = !r.greedy && r.filtered(n);
-  count[tid] = 0;
-  mass[tid] = 0;
+  for (int i = tid; i < kPlaces; i += kChunkThreads) count[i] = 0, mass[i] = 0;
   if (tid == 0) far_count = 0;
   fill_powers(powers);
   float best = -INFINITY;
@@ -238,7 +238,7 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   if (lane == 0) red_v[wave] = best, red_i[wave] = at;
   __syncthreads();
   best = red_v[0], at = red_i[0];
-  for (int i = 1; i < kWaves; ++i)
+  for (int i = 1; i < kParts; ++i)
     if (beats(red_v[i], red_i[i], best, at)) best = red_v[i], at = red_i[i];
   const size_t rc = size_t(row) * chunks + c;
   if (tid == 0) {
@@ -274,18 +274,19 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   __syncthreads();
   if (tid == 0) {
     sum = 0;
-    for (int i = 0; i < kWaves; ++i) sum += red_m[i];
+    for (int i = 0; i < kParts; ++i) sum += red_m[i];
     w.mass[rc] = sum;
   }
   if (!bins) return;
-  w.bin_count[rc * kPlaces + tid] = count[tid] + (tid == kPlaces - 1 ? far_count : 0);
-  w.bin_mass[rc * kPlaces + tid] = mass[tid];
+  for (int i = tid; i < kPlaces; i += kChunkThreads) {
+    w.bin_count[rc * kPlaces + i] = count[i] + (i == kPlaces - 1 ? far_count : 0);
+    w.bin_mass[rc * kPlaces + i] = mass[i];
+  }
 }
 
 // A chunk's weight, kept relative to its own largest logit, on the row's scale.
-__device__ __forceinline__ u64 rescale(u64 m, float chunk_top, float top, double inv, const double* powers) {
-  if (!m || chunk_top == top) return m;
-  return static_cast<u64>(rint(double(m) * weight_of(chunk_top, top, inv, powers)));
+__device__ __forceinline__ u64 rescale(u64 m, double factor) {
+  return factor == 1.0 ? m : static_cast<u64>(rint(double(m) * factor));
 }
 
 // Running sums over the workgroup's threads, own value included.
@@ -316,6 +317,8 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   __shared__ float red_v[kWaves];
   __shared__ int red_i[kWaves];
   __shared__ int found[3];
+  __shared__ double factor[kMaxChunks];
+  __shared__ int shift[kMaxChunks];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row r(s, row, n, one);
   const float* tops = w.top + size_t(row) * chunks;
@@ -350,15 +353,31 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
     return;
   }
   const double tp = place(top, r.scale);
-  for (int c = 0; c < chunks; ++c) {
-    const size_t rc = size_t(row) * chunks + c;
-    const uint32_t cc = w.bin_count[rc * kPlaces + tid];
-    if (!cc) continue;
-    const int d = tops[c] == top ? 0 : bin_below(tp, place(tops[c], r.scale));
-    const int b = min(tid + d, kPlaces - 1);
-    atomicAdd(&count[b], cc);
-    const u64 m = rescale(w.bin_mass[rc * kPlaces + tid], tops[c], top, r.inv, powers);
-    if (m) atomicAdd(&mass[b], m);
+  for (int c = tid; c < chunks; c += kThreads) {
+    const float t = tops[c];
+    factor[c] = weight_of(t, top, r.inv, powers);
+    shift[c] = t == top ? 0 : bin_below(tp, place(t, r.scale));
+  }
+  __syncthreads();
+  constexpr int kBatch = 8;
+  for (int c0 = 0; c0 < chunks; c0 += kBatch) {
+    uint32_t cc[kBatch];
+    u64 m[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const size_t at = (size_t(row) * chunks + min(c0 + j, chunks - 1)) * kPlaces + tid;
+      cc[j] = w.bin_count[at];
+      m[j] = w.bin_mass[at];
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int c = c0 + j;
+      if (c >= chunks || !cc[j]) continue;
+      const int b = min(tid + shift[c], kPlaces - 1);
+      atomicAdd(&count[b], cc[j]);
+      const u64 own = rescale(m[j], factor[c]);
+      if (own) atomicAdd(&mass[b], own);
+    }
   }
   __syncthreads();
   u64 cm = mass[tid];
@@ -430,11 +449,11 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   *st = o;
 }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kChunkThreads)
 sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
                       double one, int vec) {
   __shared__ double powers[64];
-  __shared__ u64 red_m[kWaves];
+  __shared__ u64 red_m[kChunkThreads / 64];
   __shared__ int many, next;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
   RowState* st = w.rows + row;
@@ -475,7 +494,7 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
   __syncthreads();
   if (tid == 0) {
     sum = 0;
-    for (int i = 0; i < kWaves; ++i) sum += red_m[i];
+    for (int i = 0; i < kChunkThreads / 64; ++i) sum += red_m[i];
     w.mass[rc] = sum;
     next = many ? atomicAdd(&st->listed, many) : 0;
   }
@@ -545,7 +564,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   __shared__ Digits d;
   __shared__ Entry list[kList];
   __shared__ double powers[64];
-  __shared__ u64 chunk_mass[kMaxTokens / kChunk];
+  __shared__ u64 chunk_mass[kMaxChunks];
   __shared__ u64 red_m[kWaves];
   __shared__ u64 before_of;
   __shared__ int chosen;
@@ -673,7 +692,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   if (!filtered) {
     for (int i = tid; i < chunks; i += kThreads) {
       const size_t rc = size_t(row) * chunks + i;
-      chunk_mass[i] = rescale(w.mass[rc], w.top[rc], st.top, r.inv, powers);
+      chunk_mass[i] = rescale(w.mass[rc], weight(w.top[rc]));
     }
   }
   auto kept = [&](float v, int i) -> u64 {
@@ -724,32 +743,40 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
       st.top = chunk_top;
     }
   }
-  constexpr int kPart = kChunk / kWaves;
-  const int lo = min(len, wave * kPart), hi = min(len, lo + kPart);
-  u64 m = 0;
-  for (int i = lo + lane; i < hi; i += 64) m += kept(read_logit(l[base + i]), base + i);
+  // A wave's stretch of the chunk, kPart weights a lane.
+  constexpr int kPart = kChunk / kThreads;
+  const int lo = wave * kPart * 64 + lane;
+  float v[kPart];
+#pragma unroll
+  for (int j = 0; j < kPart; ++j) v[j] = lo + 64 * j < len ? read_logit(l[base + lo + 64 * j]) : -INFINITY;
+  u64 p[kPart], m = 0;
+#pragma unroll
+  for (int j = 0; j < kPart; ++j) {
+    p[j] = kept(v[j], base + lo + 64 * j);
+    m += p[j];
+  }
   m = wave_sum(m);
   __syncthreads();
   if (lane == 0) red_m[wave] = m;
   __syncthreads();
-  u64 mine = 0;
-  for (int i = 0; i < wave; ++i) mine += red_m[i];
-  if (!(mine < want && mine + m >= want)) return;
-  u64 sum = mine;
-  for (int i0 = lo; i0 < hi; i0 += 64) {
-    const int i = i0 + lane;
-    u64 p = i < hi ? kept(read_logit(l[base + i]), base + i) : 0;
+  u64 sum = 0;
+  for (int i = 0; i < wave; ++i) sum += red_m[i];
+  if (!(sum < want && sum + m >= want)) return;
+  for (int j = 0; j < kPart; ++j) {
+    u64 q = 0;
+#pragma unroll
+    for (int i = 0; i < kPart; ++i) q = i == j ? p[i] : q;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const u64 o = __shfl_up(p, off, 64);
-      if (lane >= off) p += o;
+      const u64 o = __shfl_up(q, off, 64);
+      if (lane >= off) q += o;
     }
-    const u64 past = __ballot(sum + p >= want);
+    const u64 past = __ballot(sum + q >= want);
     if (past) {
-      if (lane == 0) out[row] = base + i0 + __ffsll(past) - 1;
+      if (lane == 0) out[row] = base + wave * kPart * 64 + 64 * j + __ffsll(past) - 1;
       return;
     }
-    sum += __shfl(p, 63, 64);
+    sum += __shfl(q, 63, 64);
   }
 }
 
@@ -774,18 +801,18 @@ extern "C" int ie_hip_sample_rows(int32_t* out, const float* logits, const float
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(IE_HIP_EINVAL, "sample_rows: needs a 16-byte aligned workspace");
   const int chunks = (n + kChunk - 1) / kChunk;
-  if (int64_t(R) * chunks * kThreads > int64_t(UINT32_MAX))
+  if (int64_t(R) * std::max(chunks * kChunkThreads, kThreads) > int64_t(UINT32_MAX))
     return fail(IE_HIP_EINVAL, "sample_rows: too many rows");
   Workspace w;
   lay_out(&w, workspace, R, n);
   const Settings s{temperature, top_k, top_p, min_p, u};
   const double one = std::ldexp(1.0, weight_bits(n));
   const int vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && n % 4 == 0;
-  const dim3 every(unsigned(R) * chunks), rows(R), block(kThreads);
-  hipLaunchKernelGGL(sample_chunks_kernel, every, block, 0, stream, logits, s, w, n, chunks, one, vec);
+  const dim3 every(unsigned(R) * chunks), rows(R), wide(kChunkThreads), block(kThreads);
+  hipLaunchKernelGGL(sample_chunks_kernel, every, wide, 0, stream, logits, s, w, n, chunks, one, vec);
   hipLaunchKernelGGL(sample_border_kernel, rows, block, 0, stream, out, s, w, n, chunks, one);
   if (top_k || top_p || min_p)
-    hipLaunchKernelGGL(sample_collect_kernel, every, block, 0, stream, logits, s, w, n, chunks, one, vec);
+    hipLaunchKernelGGL(sample_collect_kernel, every, wide, 0, stream, logits, s, w, n, chunks, one, vec);
   hipLaunchKernelGGL(sample_draw_kernel, rows, block, 0, stream, out, logits, s, w, n, chunks, one);
   return check_launch("sample_rows");
 }
