@@ -20,6 +20,7 @@
 // (64 rows x 151,936, settings mixed: one workgroup a row through all of it took 1,440 us.)
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -66,8 +67,7 @@ struct Workspace {
   RowState* rows;    // [R]
   Entry* list;       // [R, kList]
   u64* mass;         // [R, chunks] relative to the chunk's own top; after `collect` its sure weight
-  float* top;        // [R, chunks]
-  int32_t* top_at;   // [R, chunks]
+  u64* top;          // [R, chunks] the largest logit and its place (candidate)
   u64* bin_mass;     // [R, chunks, kPlaces]
   uint32_t* bin_count;
 };
@@ -84,8 +84,7 @@ size_t lay_out(Workspace* w, void* base, int R, int n) {
   v.rows = reinterpret_cast<RowState*>(take(R * sizeof(RowState)));
   v.list = reinterpret_cast<Entry*>(take(R * size_t(kList) * sizeof(Entry)));
   v.mass = reinterpret_cast<u64*>(take(rc * 8));
-  v.top = reinterpret_cast<float*>(take(rc * 4));
-  v.top_at = reinterpret_cast<int32_t*>(take(rc * 4));
+  v.top = reinterpret_cast<u64*>(take(rc * 8));
   v.bin_mass = reinterpret_cast<u64*>(take(rc * kPlaces * 8));
   v.bin_count = reinterpret_cast<uint32_t*>(take(rc * kPlaces * 4));
   if (w) *w = v;
@@ -132,9 +131,27 @@ __device__ __forceinline__ uint32_t order_key(float l) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// 2^(j / 64) in LDS, for weight_of.
+// 2^(j / 64) rounded to float64, brought to LDS for weight_of.
+__device__ const double kPowers[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0,
+};
 __device__ __forceinline__ void fill_powers(double* powers) {
-  if (threadIdx.x < 64) powers[threadIdx.x] = exp2(double(threadIdx.x) / 64.0);
+  if (threadIdx.x < 64) powers[threadIdx.x] = kPowers[threadIdx.x];
 }
 
 // exp((l - top) / T) in [0, 1]. With m = round(64 x / ln 2) and r = x - m ln2 / 64, |r| <= 0.0055:
@@ -193,15 +210,52 @@ __device__ __forceinline__ void load_chunk(float (&v)[kEach], const float* l, in
   for (int j = 0; j < kEach; ++j) v[j] = read_logit(v[j]);
 }
 
-__device__ __forceinline__ u64 wave_sum(u64 m) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m += __shfl_xor(m, off, 64);
-  return m;
+// Running sums and maxima over a wave's lanes with the VALU's lane shifts (each row of 16 by 1, 2, 4 and
+// 8, then rows 0 into 1 and 2 into 3, then lane 31 into the upper half): a step takes a few cycles, a
+// shuffle through LDS some hundred.
+template <int CTRL, int ROWS, class T, class F>
+__device__ __forceinline__ T lane_step(T x, const F& join) {
+  T y;
+  if constexpr (sizeof(T) == 8) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(x)), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(x >> 32)), CTRL, ROWS, 0xF, false);
+    y = T(hi) << 32 | lo;
+  } else {
+    y = __builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xF, false);
+  }
+  return join(x, y);  // lanes without a source join 0
 }
+template <class T, class F>
+__device__ __forceinline__ T wave_scan(T x, const F& join) {
+  x = lane_step<0x111, 0xF>(x, join);  // row_shr:1
+  x = lane_step<0x112, 0xF>(x, join);
+  x = lane_step<0x114, 0xF>(x, join);
+  x = lane_step<0x118, 0xF>(x, join);
+  x = lane_step<0x142, 0xA>(x, join);  // row_bcast:15 into rows 1 and 3
+  return lane_step<0x143, 0xC>(x, join);  // row_bcast:31 into rows 2 and 3
+}
+template <class T>
+__device__ __forceinline__ T wave_running(T x) {
+  return wave_scan(x, [](T a, T b) { return a + b; });
+}
+__device__ __forceinline__ u64 last_lane(u64 x) {
+  return u64(uint32_t(__builtin_amdgcn_readlane(int(x >> 32), 63))) << 32 |
+         uint32_t(__builtin_amdgcn_readlane(int(x), 63));
+}
+__device__ __forceinline__ u64 wave_sum(u64 m) { return last_lane(wave_running(m)); }
 
-__device__ __forceinline__ bool beats(float v, int i, float best, int at) {
-  return v > best || (v == best && i < at);
+// A logit and its place as one number: larger logits, then lower places, are larger; 0 is none.
+__device__ __forceinline__ u64 candidate(float l, int i) {
+  return l > -INFINITY ? u64(order_key(l)) << 32 | uint32_t(~i) : 0;
 }
+__device__ __forceinline__ u64 wave_best(u64 c) {
+  return last_lane(wave_scan(c, [](u64 a, u64 b) { return a > b ? a : b; }));
+}
+__device__ __forceinline__ float candidate_logit(u64 c) {
+  const uint32_t o = uint32_t(c >> 32);
+  return !c ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ int candidate_place(u64 c) { return int(~uint32_t(c)); }
 
 __global__ void __launch_bounds__(kChunkThreads)
 sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
@@ -210,9 +264,7 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   __shared__ uint32_t count[kPlaces];
   __shared__ u64 mass[kPlaces];
   __shared__ double powers[64];
-  __shared__ float red_v[kParts];
-  __shared__ int red_i[kParts];
-  __shared__ u64 red_m[kParts];
+  __shared__ u64 red_m[kParts], red_s[kParts];
   __shared__ uint32_t far_count;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -224,27 +276,21 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   for (int i = tid; i < kPlaces; i += kChunkThreads) count[i] = 0, mass[i] = 0;
   if (tid == 0) far_count = 0;
   fill_powers(powers);
-  float best = -INFINITY;
-  int at = 0x7fffffff;
+  u64 found = 0;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j)
-    if (v[j] > best) best = v[j], at = chunk_index(j);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const float o = __shfl_xor(best, off, 64);
-    const int i = __shfl_xor(at, off, 64);
-    if (beats(o, i, best, at)) best = o, at = i;
+  for (int j = 0; j < kEach; ++j) {
+    const u64 c = candidate(v[j], base + chunk_index(j));
+    found = c > found ? c : found;
   }
-  if (lane == 0) red_v[wave] = best, red_i[wave] = at;
+  found = wave_best(found);
+  if (lane == 0) red_m[wave] = found;
   __syncthreads();
-  best = red_v[0], at = red_i[0];
-  for (int i = 1; i < kParts; ++i)
-    if (beats(red_v[i], red_i[i], best, at)) best = red_v[i], at = red_i[i];
+  found = 0;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) found = red_m[i] > found ? red_m[i] : found;
+  const float best = candidate_logit(found);
   const size_t rc = size_t(row) * chunks + c;
-  if (tid == 0) {
-    w.top[rc] = best;
-    w.top_at[rc] = best > -INFINITY ? base + at : 0x7fffffff;
-  }
+  if (tid == 0) w.top[rc] = found;
   if (r.greedy) return;
   u64 sum = 0;
   uint32_t far = 0;
@@ -265,16 +311,16 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
     }
   }
   sum = wave_sum(sum);
-  if (lane == 0) red_m[wave] = sum;
+  if (lane == 0) red_s[wave] = sum;
   if (bins) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) far += __shfl_xor(far, off, 64);
+    far = __builtin_amdgcn_readlane(wave_running(far), 63);
     if (lane == 0 && far) atomicAdd(&far_count, far);
   }
   __syncthreads();
   if (tid == 0) {
     sum = 0;
-    for (int i = 0; i < kParts; ++i) sum += red_m[i];
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) sum += red_s[i];
     w.mass[rc] = sum;
   }
   if (!bins) return;
@@ -290,22 +336,16 @@ __device__ __forceinline__ u64 rescale(u64 m, double factor) {
 }
 
 // Running sums over the workgroup's threads, own value included.
-struct Scan {
-  u64 mass[kWaves];
-  uint32_t count[kWaves];
-};
-__device__ __forceinline__ void scan(Scan& sh, u64& m, uint32_t& c) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <class T>
+__device__ __forceinline__ T running(u64 (&sh)[kWaves], T x) {
+  const int wave = threadIdx.x >> 6;
+  x = wave_running(x);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) sh[wave] = x;
+  __syncthreads();
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const u64 om = __shfl_up(m, off, 64);
-    const uint32_t oc = __shfl_up(c, off, 64);
-    if (lane >= off) m += om, c += oc;
-  }
-  __syncthreads();
-  if (lane == 63) sh.mass[wave] = m, sh.count[wave] = c;
-  __syncthreads();
-  for (int i = 0; i < wave; ++i) m += sh.mass[i], c += sh.count[i];
+  for (int i = 0; i < kWaves; ++i) x += i < wave ? T(sh[i]) : T(0);
+  return x;
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -313,62 +353,59 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   __shared__ uint32_t count[kPlaces];
   __shared__ u64 mass[kPlaces];
   __shared__ double powers[64];
-  __shared__ Scan sh;
-  __shared__ float red_v[kWaves];
-  __shared__ int red_i[kWaves];
+  __shared__ u64 sh[kWaves];
   __shared__ int found[3];
   __shared__ double factor[kMaxChunks];
   __shared__ int shift[kMaxChunks];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row r(s, row, n, one);
-  const float* tops = w.top + size_t(row) * chunks;
-  count[tid] = 0;
-  mass[tid] = 0;
-  if (tid < 3) found[tid] = kPlaces - 1;
-  fill_powers(powers);
-  float top = -INFINITY;
-  int at = 0x7fffffff;
-  for (int c = tid; c < chunks; c += kThreads) {
-    const int i = w.top_at[size_t(row) * chunks + c];
-    if (beats(tops[c], i, top, at)) top = tops[c], at = i;
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const float o = __shfl_xor(top, off, 64);
-    const int i = __shfl_xor(at, off, 64);
-    if (beats(o, i, top, at)) top = o, at = i;
-  }
-  if (lane == 0) red_v[wave] = top, red_i[wave] = at;
-  __syncthreads();
-  top = red_v[0], at = red_i[0];
-  for (int i = 1; i < kWaves; ++i)
-    if (beats(red_v[i], red_i[i], top, at)) top = red_v[i], at = red_i[i];
-  RowState* st = w.rows + row;
-  if (r.greedy || at == 0x7fffffff || !r.filtered(n)) {
-    if (tid == 0) {
-      st->mode = r.greedy || at == 0x7fffffff ? kDone : kAll;
-      st->top = top;
-      if (st->mode == kDone) out[row] = at == 0x7fffffff ? 0 : at;
-    }
-    return;
-  }
-  const double tp = place(top, r.scale);
-  for (int c = tid; c < chunks; c += kThreads) {
-    const float t = tops[c];
-    factor[c] = weight_of(t, top, r.inv, powers);
-    shift[c] = t == top ? 0 : bin_below(tp, place(t, r.scale));
-  }
-  __syncthreads();
-  constexpr int kBatch = 8;
-  for (int c0 = 0; c0 < chunks; c0 += kBatch) {
-    uint32_t cc[kBatch];
-    u64 m[kBatch];
+  const u64* tops = w.top + size_t(row) * chunks;
+  // The first chunks' histograms, on their way while the row's largest logit is found.
+  constexpr int kBatch = 20;
+  uint32_t cc[kBatch];
+  u64 m[kBatch];
+  auto fetch = [&](int c0) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const size_t at = (size_t(row) * chunks + min(c0 + j, chunks - 1)) * kPlaces + tid;
       cc[j] = w.bin_count[at];
       m[j] = w.bin_mass[at];
     }
+  };
+  const bool bins = !r.greedy && r.filtered(n);
+  if (bins) fetch(0);
+  count[tid] = 0;
+  mass[tid] = 0;
+  if (tid < 3) found[tid] = kPlaces - 1;
+  fill_powers(powers);
+  u64 best = 0;
+  for (int c = tid; c < chunks; c += kThreads) best = tops[c] > best ? tops[c] : best;
+  best = wave_best(best);
+  if (lane == 0) sh[wave] = best;
+  __syncthreads();
+  best = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) best = sh[i] > best ? sh[i] : best;
+  const float top = candidate_logit(best);
+  RowState* st = w.rows + row;
+  if (!bins || !best) {
+    if (tid == 0) {
+      const bool done = r.greedy || !best;
+      st->mode = done ? kDone : kAll;
+      st->top = top;
+      if (done) out[row] = best ? candidate_place(best) : 0;
+    }
+    return;
+  }
+  const double tp = place(top, r.scale);
+  for (int c = tid; c < chunks; c += kThreads) {
+    const float t = candidate_logit(tops[c]);
+    factor[c] = weight_of(t, top, r.inv, powers);
+    shift[c] = t == top ? 0 : bin_below(tp, place(t, r.scale));
+  }
+  __syncthreads();
+  for (int c0 = 0; c0 < chunks; c0 += kBatch) {
+    if (c0 > 0) fetch(c0);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
       const int c = c0 + j;
@@ -380,11 +417,10 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
     }
   }
   __syncthreads();
-  u64 cm = mass[tid];
-  uint32_t cn = count[tid];
-  const uint32_t own_n = cn;
-  const u64 own_m = cm;
-  scan(sh, cm, cn);
+  const uint32_t own_n = count[tid];
+  const u64 own_m = mass[tid];
+  const u64 cm = running(sh, own_m);
+  const uint32_t cn = running(sh, own_n);
   __syncthreads();
   count[tid] = cn;  // running sums from here on
   mass[tid] = cm;
@@ -462,7 +498,7 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
   const size_t rc = size_t(row) * chunks + c;
   const int sure = st->sure, outer_lo = st->outer_lo, outer_hi = st->outer_hi;
   const int inner_lo = st->inner_lo, inner_hi = st->inner_hi;
-  const float top = st->top, chunk_top = w.top[rc];
+  const float top = st->top, chunk_top = candidate_logit(w.top[rc]);
   const Row r(s, row, n, one);
   const double tp = place(top, r.scale);
   const int nearest = chunk_top == top ? 0 : bin_below(tp, place(chunk_top, r.scale));
@@ -512,19 +548,24 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
 struct Digits {
   u64 mass[kDigits];
   uint32_t count[kDigits];
-  Scan scan;
+  u64 sums[kWaves];
   int bin;
-  uint32_t before_count, in_count;
-  u64 before_mass;
+  uint32_t in_count;
+  u64 before;
 };
 
-// One digit over `items` tokens: digit(i, mass) gives a token's bin (-1: none) and weight; the bin
-// in which reach(running count, running mass) first holds is left in d (d.bin = -1: in none).
-template <class Digit, class Reach>
+// One digit over `items` tokens: digit(i, mass) gives a token's bin (-1: none) and weight. The bin in
+// which reach(running sum) first holds, of the weights with MASS, of the counts otherwise, is left in d
+// (d.bin = -1: in none) with the sum before it.
+template <bool MASS, class Digit, class Reach>
 __device__ __forceinline__ void digit_pass(Digits& d, int items, const Digit& digit, const Reach& reach) {
   const int tid = threadIdx.x;
   __syncthreads();
-  for (int i = tid; i < kDigits; i += kThreads) d.mass[i] = 0, d.count[i] = 0;
+#pragma unroll
+  for (int i = 0; i < kDigits / kThreads; ++i) {
+    d.count[i * kThreads + tid] = 0;
+    if (MASS) d.mass[i * kThreads + tid] = 0;
+  }
   if (tid == 0) d.bin = -1;
   __syncthreads();
   for (int i0 = 0; i0 < items; i0 += kThreads) {
@@ -534,27 +575,23 @@ __device__ __forceinline__ void digit_pass(Digits& d, int items, const Digit& di
     const int first = __builtin_amdgcn_readfirstlane(b);
     if (__all(b == first)) {
       if (first < 0) continue;
-      m = wave_sum(m);
+      if (MASS) m = wave_sum(m);
       if ((tid & 63) == 0) {
         atomicAdd(&d.count[first], 64u);
-        if (m) atomicAdd(&d.mass[first], m);
+        if (MASS && m) atomicAdd(&d.mass[first], m);
       }
     } else if (b >= 0) {
       atomicAdd(&d.count[b], 1u);
-      if (m) atomicAdd(&d.mass[b], m);
+      if (MASS && m) atomicAdd(&d.mass[b], m);
     }
   }
   __syncthreads();
   const uint32_t n0 = d.count[2 * tid], n1 = d.count[2 * tid + 1];
-  const u64 m0 = d.mass[2 * tid], m1 = d.mass[2 * tid + 1];
-  u64 cm = m0 + m1;
-  uint32_t cn = n0 + n1;
-  scan(d.scan, cm, cn);
-  const u64 bm = cm - m0 - m1;
-  const uint32_t bn = cn - n0 - n1;
-  const bool r0 = reach(bn, bm), r1 = reach(bn + n0, bm + m0), r2 = reach(cn, cm);
-  if (!r0 && r1) d.bin = 2 * tid, d.before_count = bn, d.before_mass = bm, d.in_count = n0;
-  if (!r1 && r2) d.bin = 2 * tid + 1, d.before_count = bn + n0, d.before_mass = bm + m0, d.in_count = n1;
+  const u64 s0 = MASS ? d.mass[2 * tid] : n0, s1 = MASS ? d.mass[2 * tid + 1] : n1;
+  const u64 sum = running(d.sums, s0 + s1), before = sum - s0 - s1;
+  const bool r0 = reach(before), r1 = reach(before + s0), r2 = reach(sum);
+  if (!r0 && r1) d.bin = 2 * tid, d.before = before, d.in_count = n0;
+  if (!r1 && r2) d.bin = 2 * tid + 1, d.before = before + s0, d.in_count = n1;
   __syncthreads();
 }
 
@@ -605,14 +642,16 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   auto stays = [&](float v, int i, int b, double e) {
     return b <= end && above(v, i) && (!outer(b) || e >= r.least);
   };
-  // Moves (key, last) to the token at which reach() first holds of the running sums over the tokens
-  // that `take` lets in; `stay` says how many of the last key's equal tokens that is.
-  auto select = [&](const auto& take, const auto& reach, const auto& stay) {
-    uint32_t prefix = 0, n0 = 0;
-    u64 m0 = 0;
+  // Moves (key, last) to the token at which reach() first holds of the running sums (of weights with
+  // by_mass, else of tokens) over the tokens that `take` lets in; stay() says how many of the last key's
+  // equal tokens that is.
+  auto select = [&](auto by_mass, const auto& take, const auto& reach, const auto& stay) {
+    constexpr bool MASS = decltype(by_mass)::value;
+    uint32_t prefix = 0;
+    u64 sum = 0;
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      digit_pass(
+      digit_pass<MASS>(
           d, items,
           [&](int i, u64& m) {
             const Entry e = entry(i);
@@ -620,30 +659,27 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
             if (pass > 0 && (o >> (shift + bits)) != prefix) return -1;
             return take(e.l, e.i, m) ? int(((1u << bits) - 1) - ((o >> shift) & ((1u << bits) - 1))) : -1;
           },
-          [&](uint32_t c, u64 m) { return reach(n0 + c, m0 + m); });
+          [&](u64 s) { return reach(sum + s); });
       if (d.bin < 0) return;  // never: all stay
       prefix = (prefix << bits) | (((1u << bits) - 1) - uint32_t(d.bin));
-      n0 += d.before_count;
-      m0 += d.before_mass;
+      sum += d.before;
     }
-    const uint32_t equal = d.in_count, keep = equal > 1 ? stay(equal, n0, m0, prefix) : 1;
+    const uint32_t equal = d.in_count, keep = equal > 1 ? stay(equal, sum, prefix) : 1;
     int to = 0x7fffffff;
     if (keep < equal) {  // the index of the keep-th of them
       int high = 0;
-      uint32_t c0 = 0;
+      u64 c0 = 0;
       for (int pass = 0; pass < 2; ++pass) {
-        digit_pass(
+        digit_pass<false>(
             d, items,
-            [&](int i, u64& m) {
+            [&](int i, u64&) {
               const Entry e = entry(i);
               if (order_key(e.l) != prefix || (pass == 1 && e.i >> 11 != high)) return -1;
-              const int at = pass == 0 ? e.i >> 11 : e.i & 2047;
-              const bool in = take(e.l, e.i, m);
-              m = 0;
-              return in ? at : -1;
+              u64 m;
+              return take(e.l, e.i, m) ? (pass == 0 ? e.i >> 11 : e.i & 2047) : -1;
             },
-            [&](uint32_t c, u64) { return c0 + c >= keep; });
-        if (pass == 0) high = d.bin, c0 = d.before_count;
+            [&](u64 c) { return c0 + c >= keep; });
+        if (pass == 0) high = d.bin, c0 = d.before;
       }
       to = (high << 11) | d.bin;
     }
@@ -653,35 +689,41 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
 
   if (filtered && st.top_left != 0x7fffffff) {
     const uint32_t left = uint32_t(st.top_left);
-    select([&](float v, int, u64&) { return outer(bin_of(v)); },
-           [&](uint32_t c, u64) { return c >= left; },
-           [&](uint32_t, uint32_t c, u64, uint32_t) { return left - c; });
+    select(
+        std::false_type{}, [&](float v, int, u64&) { return outer(bin_of(v)); },
+        [&](u64 c) { return c >= left; },
+        [&](uint32_t, u64 c, uint32_t) { return left - uint32_t(c); });
   }
   if (filtered && r.p < 1.0f) {
-    u64 m = 0;
-    for (int i = tid; i < items; i += kThreads) {
-      const Entry e = entry(i);
-      const int b = bin_of(e.l);
-      const double x = weight(e.l);
-      if (outer(b) && stays(e.l, e.i, b, x)) m += whole(x, one);
+    u64 of = st.total;
+    if (st.outer_lo < kPlaces) {
+      u64 m = 0;
+      for (int i = tid; i < items; i += kThreads) {
+        const Entry e = entry(i);
+        const int b = bin_of(e.l);
+        const double x = weight(e.l);
+        if (outer(b) && stays(e.l, e.i, b, x)) m += whole(x, one);
+      }
+      m = wave_sum(m);
+      __syncthreads();
+      if (lane == 0) red_m[wave] = m;
+      __syncthreads();
+      of = st.outer_mass;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) of += red_m[i];
     }
-    m = wave_sum(m);
-    __syncthreads();
-    if (lane == 0) red_m[wave] = m;
-    __syncthreads();
-    u64 of = st.outer_lo < kPlaces ? st.outer_mass : st.total;
-    for (int i = 0; i < kWaves; ++i) of += red_m[i];
     const double goal = double(r.p) * double(of);
     end = st.inner_hi;
     select(
+        std::true_type{},
         [&](float v, int i, u64& m) {
           const int b = bin_of(v);
           const double x = weight(v);
           m = whole(x, one);
           return stays(v, i, b, x);
         },
-        [&](uint32_t, u64 m) { return double(st.sure_mass + m) >= goal; },
-        [&](uint32_t equal, uint32_t, u64 m, uint32_t o) {
+        [&](u64 m) { return double(st.sure_mass + m) >= goal; },
+        [&](uint32_t equal, u64 m, uint32_t o) {
           const float v = __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
           const double each = double(whole(weight(v), one));
           const double need = (goal - double(st.sure_mass + m)) / each;
@@ -692,7 +734,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   if (!filtered) {
     for (int i = tid; i < chunks; i += kThreads) {
       const size_t rc = size_t(row) * chunks + i;
-      chunk_mass[i] = rescale(w.mass[rc], weight(w.top[rc]));
+      chunk_mass[i] = rescale(w.mass[rc], weight(candidate_logit(w.top[rc])));
     }
   }
   auto kept = [&](float v, int i) -> u64 {
@@ -718,10 +760,8 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
     }
   }
   __syncthreads();
-  u64 cm = tid < chunks ? chunk_mass[tid] : 0;
-  const u64 own = cm;
-  uint32_t unused = 0;
-  scan(d.scan, cm, unused);
+  const u64 own = tid < chunks ? chunk_mass[tid] : 0;
+  const u64 cm = running(d.sums, own);
   if (tid == kThreads - 1) before_of = cm;
   __syncthreads();
   const u64 total = before_of;
@@ -736,7 +776,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   u64 want = need - before_of;
   if (!filtered) {  // in the chunk's own units, whose sum is at hand
     const size_t rc = size_t(row) * chunks + chosen;
-    const float chunk_top = w.top[rc];
+    const float chunk_top = candidate_logit(w.top[rc]);
     if (chunk_top != st.top) {
       const double f = weight(chunk_top);
       want = max(u64(1), min(w.mass[rc], static_cast<u64>(ceil(double(want) / f))));
@@ -760,23 +800,20 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   if (lane == 0) red_m[wave] = m;
   __syncthreads();
   u64 sum = 0;
-  for (int i = 0; i < wave; ++i) sum += red_m[i];
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) sum += i < wave ? red_m[i] : 0;
   if (!(sum < want && sum + m >= want)) return;
   for (int j = 0; j < kPart; ++j) {
     u64 q = 0;
 #pragma unroll
     for (int i = 0; i < kPart; ++i) q = i == j ? p[i] : q;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const u64 o = __shfl_up(q, off, 64);
-      if (lane >= off) q += o;
-    }
+    q = wave_running(q);
     const u64 past = __ballot(sum + q >= want);
     if (past) {
       if (lane == 0) out[row] = base + wave * kPart * 64 + 64 * j + __ffsll(past) - 1;
       return;
     }
-    sum += __shfl(q, 63, 64);
+    sum += last_lane(q);
   }
 }
 
