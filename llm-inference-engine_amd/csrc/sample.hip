@@ -43,7 +43,7 @@ int weight_bits(int n) {
   return std::min(45, 63 - log2);
 }
 
-enum Mode { kDone, kAll, kFiltered, kWhole };
+enum Mode { kDone, kAll, kFiltered };
 
 // What the border launch leaves of a row. Bins below `sure` are kept whole; those in
 // [outer_lo, outer_hi] hold the border of top-k or min-p, those in [inner_lo, inner_hi] top-p's.
@@ -265,16 +265,13 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   __shared__ u64 mass[kPlaces];
   __shared__ double powers[64];
   __shared__ u64 red_m[kParts], red_s[kParts];
-  __shared__ uint32_t far_count;
   const int row = blockIdx.x / chunks, c = blockIdx.x - row * chunks;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int base = c * kChunk, len = min(kChunk, n - base);
   float v[kEach];
   load_chunk(v, logits + size_t(row) * n + base, len, vec);
   const Row r(s, row, n, one);
-  const bool bins = !r.greedy && r.filtered(n);
   for (int i = tid; i < kPlaces; i += kChunkThreads) count[i] = 0, mass[i] = 0;
-  if (tid == 0) far_count = 0;
   fill_powers(powers);
   u64 found = 0;
 #pragma unroll
@@ -291,31 +288,23 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   const float best = candidate_logit(found);
   const size_t rc = size_t(row) * chunks + c;
   if (tid == 0) w.top[rc] = found;
-  if (r.greedy) return;
+  const bool by_count = r.k < n, by_mass = r.p < 1.0f;
+  if (r.greedy || (r.filtered(n) && !by_count && !by_mass)) return;  // min-p alone needs no sums here
   u64 sum = 0;
-  uint32_t far = 0;
   const double tp = place(best, r.scale);
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    if (chunk_index(j) >= len) continue;
-    const u64 m = v[j] == -INFINITY ? 0 : whole(weight_of(v[j], best, r.inv, powers), one);
+    if (v[j] == -INFINITY) continue;  // (a masked row's tokens, and what is past the row)
+    const u64 m = by_count && !by_mass ? 0 : whole(weight_of(v[j], best, r.inv, powers), one);
     sum += m;
-    if (!bins) continue;
+    if (!by_count && !by_mass) continue;
     const int b = v[j] == best ? 0 : bin_below(tp, place(v[j], r.scale));
-    if (b == kPlaces - 1) {
-      ++far;  // a masked row's tokens: not one by one
-      if (m) atomicAdd(&mass[b], m);
-    } else {
-      atomicAdd(&count[b], 1u);
-      atomicAdd(&mass[b], m);
-    }
+    if (b == kPlaces - 1) continue;  // what the others leave
+    if (by_count) atomicAdd(&count[b], 1u);
+    if (by_mass) atomicAdd(&mass[b], m);
   }
   sum = wave_sum(sum);
   if (lane == 0) red_s[wave] = sum;
-  if (bins) {
-    far = __builtin_amdgcn_readlane(wave_running(far), 63);
-    if (lane == 0 && far) atomicAdd(&far_count, far);
-  }
   __syncthreads();
   if (tid == 0) {
     sum = 0;
@@ -323,11 +312,10 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
     for (int i = 0; i < kParts; ++i) sum += red_s[i];
     w.mass[rc] = sum;
   }
-  if (!bins) return;
-  for (int i = tid; i < kPlaces; i += kChunkThreads) {
-    w.bin_count[rc * kPlaces + i] = count[i] + (i == kPlaces - 1 ? far_count : 0);
-    w.bin_mass[rc * kPlaces + i] = mass[i];
-  }
+  if (by_count)
+    for (int i = tid; i < kPlaces; i += kChunkThreads) w.bin_count[rc * kPlaces + i] = count[i];
+  if (by_mass)
+    for (int i = tid; i < kPlaces; i += kChunkThreads) w.bin_mass[rc * kPlaces + i] = mass[i];
 }
 
 // A chunk's weight, kept relative to its own largest logit, on the row's scale.
@@ -360,22 +348,6 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row r(s, row, n, one);
   const u64* tops = w.top + size_t(row) * chunks;
-  // The first chunks' histograms, on their way while the row's largest logit is found.
-  constexpr int kBatch = 20;
-  uint32_t cc[kBatch];
-  u64 m[kBatch];
-  auto fetch = [&](int c0) {
-#pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const size_t at = (size_t(row) * chunks + min(c0 + j, chunks - 1)) * kPlaces + tid;
-      cc[j] = w.bin_count[at];
-      m[j] = w.bin_mass[at];
-    }
-  };
-  const bool bins = !r.greedy && r.filtered(n);
-  if (bins) fetch(0);
-  count[tid] = 0;
-  mass[tid] = 0;
   if (tid < 3) found[tid] = kPlaces - 1;
   fill_powers(powers);
   u64 best = 0;
@@ -388,7 +360,7 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   for (int i = 0; i < kWaves; ++i) best = sh[i] > best ? sh[i] : best;
   const float top = candidate_logit(best);
   RowState* st = w.rows + row;
-  if (!bins || !best) {
+  if (r.greedy || !best || !r.filtered(n)) {
     if (tid == 0) {
       const bool done = r.greedy || !best;
       st->mode = done ? kDone : kAll;
@@ -404,24 +376,40 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
     shift[c] = t == top ? 0 : bin_below(tp, place(t, r.scale));
   }
   __syncthreads();
+  // This thread's bin over the chunks: each has it further down by how far its own top is below the
+  // row's. The last bin is what the others leave, so nothing is added up from several bins.
+  const bool by_count = r.k < n, by_mass = r.p < 1.0f;
+  u64 own_m = 0, all = 0;
+  uint32_t own_n = 0;
+  constexpr int kBatch = 8;
   for (int c0 = 0; c0 < chunks; c0 += kBatch) {
-    if (c0 > 0) fetch(c0);
+    uint32_t cc[kBatch];
+    u64 m[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      const int c = c0 + j;
-      if (c >= chunks || !cc[j]) continue;
-      const int b = min(tid + shift[c], kPlaces - 1);
-      atomicAdd(&count[b], cc[j]);
-      const u64 own = rescale(m[j], factor[c]);
-      if (own) atomicAdd(&mass[b], own);
+      const int c = min(c0 + j, chunks - 1), bin = tid - shift[c];
+      const bool in = c0 + j < chunks && bin >= 0;
+      const size_t at = (size_t(row) * chunks + c) * kPlaces + (in ? bin : 0);
+      cc[j] = in && by_count ? w.bin_count[at] : 0;
+      m[j] = in && by_mass ? w.bin_mass[at] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      own_n += cc[j];
+      own_m += rescale(m[j], factor[min(c0 + j, chunks - 1)]);
     }
   }
-  __syncthreads();
-  const uint32_t own_n = count[tid];
-  const u64 own_m = mass[tid];
-  const u64 cm = running(sh, own_m);
-  const uint32_t cn = running(sh, own_n);
-  __syncthreads();
+  if (by_mass)
+    for (int c = 0; c < chunks; ++c) all += rescale(w.mass[size_t(row) * chunks + c], factor[c]);
+  if (tid == kPlaces - 1) own_m = 0, own_n = 0;
+  u64 cm = by_mass ? running(sh, own_m) : 0;
+  uint32_t cn = by_count ? running(sh, own_n) : 0;
+  if (tid == kPlaces - 1) {
+    own_m = all > cm ? all - cm : 0;
+    own_n = uint32_t(n) - cn;
+    cm += own_m;
+    cn = uint32_t(n);
+  }
   count[tid] = cn;  // running sums from here on
   mass[tid] = cm;
   const u64 bm = cm - own_m;
@@ -429,7 +417,6 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   // top-k's bin: the one in which the running count reaches k
   if (bn < uint32_t(r.k) && cn >= uint32_t(r.k)) found[0] = tid;
   __syncthreads();
-  const bool by_count = r.k < n;
   int lo = 0x7fffffff, hi = -1, left = 0x7fffffff;
   if (r.least > 0.0) {
     // min-p's: one bin to either side of where its logit falls, for the roundings of the two
@@ -473,15 +460,7 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   o.top_left = left;
   o.pad = 0;
   o.listed = 0;
-  auto between = [&](int a, int b) { return a >= kPlaces ? 0u : count[b] - (a ? count[a - 1] : 0u); };
-  uint32_t many = between(o.outer_lo, o.outer_hi);
-  if (o.inner_lo < kPlaces) {
-    if (o.outer_lo >= kPlaces || o.inner_hi < o.outer_lo)
-      many += between(o.inner_lo, o.inner_hi);
-    else if (o.inner_lo < o.outer_lo)
-      many = between(o.inner_lo, o.outer_hi);
-  }
-  o.mode = many <= uint32_t(kList) ? kFiltered : kWhole;
+  o.mode = kFiltered;
   *st = o;
 }
 
@@ -610,7 +589,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   if (st.mode == kDone) return;
   const float* l = logits + size_t(row) * n;
   const Row r(s, row, n, one);
-  const bool filtered = st.mode != kAll, all = st.mode == kWhole;
+  const bool filtered = st.mode != kAll, all = filtered && st.listed > kList;
   const double tp = place(st.top, r.scale);
   fill_powers(powers);
   if (all) {
@@ -618,7 +597,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
     st.sure_mass = st.outer_mass = 0;
     st.top_left = r.k < n ? r.k : 0x7fffffff;
   }
-  const int items = !filtered ? 0 : all ? n : min(st.listed, kList);
+  const int items = !filtered ? 0 : all ? n : st.listed;
   if (filtered && !all)
     for (int i = tid; i < items; i += kThreads) list[i] = w.list[size_t(row) * kList + i];
   for (int i = tid; i < chunks; i += kThreads) {
@@ -626,6 +605,21 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
     chunk_mass[i] = filtered && !all ? w.mass[rc] : 0;
   }
   __syncthreads();
+  // The list's logits agree in their leading bits, being of few bins: how many digits that leaves.
+  int digits = 3;
+  uint32_t common_prefix = 0;
+  if (filtered && !all && items > 0) {
+    const uint32_t o = order_key(list[0].l);
+    uint32_t differ = 0;
+    for (int i = tid; i < items; i += kThreads) differ |= order_key(list[i].l) ^ o;
+    if (tid == 0) chosen = 0;
+    __syncthreads();
+    if (differ) atomicOr(&chosen, int(differ));
+    __syncthreads();
+    const uint32_t any = uint32_t(chosen);
+    digits = any >> 21 ? 3 : any >> 10 ? 2 : 1;
+    common_prefix = digits == 3 ? 0 : digits == 2 ? o >> 21 : o >> 10;
+  }
   auto entry = [&](int i) { return all ? Entry{read_logit(l[i]), i} : list[i]; };
   auto bin_of = [&](float v) { return v == st.top ? 0 : bin_below(tp, place(v, r.scale)); };
   auto weight = [&](float v) { return weight_of(v, st.top, r.inv, powers); };
@@ -647,16 +641,16 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   // equal tokens that is.
   auto select = [&](auto by_mass, const auto& take, const auto& reach, const auto& stay) {
     constexpr bool MASS = decltype(by_mass)::value;
-    uint32_t prefix = 0;
+    uint32_t prefix = common_prefix;
     u64 sum = 0;
-    for (int pass = 0; pass < 3; ++pass) {
+    for (int pass = 3 - digits; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
       digit_pass<MASS>(
           d, items,
           [&](int i, u64& m) {
             const Entry e = entry(i);
             const uint32_t o = order_key(e.l);
-            if (pass > 0 && (o >> (shift + bits)) != prefix) return -1;
+            if (pass > 3 - digits && (o >> (shift + bits)) != prefix) return -1;
             return take(e.l, e.i, m) ? int(((1u << bits) - 1) - ((o >> shift) & ((1u << bits) - 1))) : -1;
           },
           [&](u64 s) { return reach(sum + s); });
