@@ -30,15 +30,13 @@ adjust_logits_kernel(float* out, const float* logits, ie_logit_rules u, int n, i
   float4 l[kQuads];
 #pragma unroll
   for (int q = 0; q < kQuads; ++q) {
+    // (past the end: some logit of the segment, never stored; a load behind a condition would wait)
     const int i = quad(q);
-    if constexpr (VEC) {  // n and so len are multiples of 4
-      l[q] = i < len ? *reinterpret_cast<const float4*>(logits + at + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    } else {
-      l[q].x = i < len ? logits[at + i] : 0.f;
-      l[q].y = i + 1 < len ? logits[at + i + 1] : 0.f;
-      l[q].z = i + 2 < len ? logits[at + i + 2] : 0.f;
-      l[q].w = i + 3 < len ? logits[at + i + 3] : 0.f;
-    }
+    if constexpr (VEC)  // n and so len are multiples of 4
+      l[q] = *reinterpret_cast<const float4*>(logits + at + min(i, len - 4));
+    else
+      l[q] = make_float4(logits[at + min(i, len - 1)], logits[at + min(i + 1, len - 1)],
+                         logits[at + min(i + 2, len - 1)], logits[at + min(i + 3, len - 1)]);
   }
   auto clear = [&]() {
 #pragma unroll

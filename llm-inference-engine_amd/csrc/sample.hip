@@ -194,20 +194,23 @@ __device__ __forceinline__ float read_logit(float v) { return v == v ? v : -INFI
 __device__ __forceinline__ int chunk_index(int j) {
   return ((j >> 2) * kChunkThreads + int(threadIdx.x)) * 4 + (j & 3);
 }
-__device__ __forceinline__ void load_chunk(float (&v)[kEach], const float* l, int len, bool vec) {
+// VEC: n is a multiple of 4. Every load is issued, at a place within the chunk, and what is past its end
+// replaced: a load behind a condition would wait for the one before.
+template <bool VEC>
+__device__ __forceinline__ void load_chunk(float (&v)[kEach], const float* l, int len) {
 #pragma unroll
   for (int u = 0; u < kEach / 4; ++u) {
     const int at = chunk_index(4 * u);
-    if (vec && at + 3 < len) {
-      const float4 q = *reinterpret_cast<const float4*>(l + at);
+    if constexpr (VEC) {
+      const float4 q = *reinterpret_cast<const float4*>(l + min(at, len - 4));
       v[4 * u] = q.x, v[4 * u + 1] = q.y, v[4 * u + 2] = q.z, v[4 * u + 3] = q.w;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * u + e] = at + e < len ? l[at + e] : -INFINITY;
+      for (int e = 0; e < 4; ++e) v[4 * u + e] = l[min(at + e, len - 1)];
     }
   }
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) v[j] = read_logit(v[j]);
+  for (int j = 0; j < kEach; ++j) v[j] = chunk_index(j) < len ? read_logit(v[j]) : -INFINITY;
 }
 
 // Running sums and maxima over a wave's lanes with the VALU's lane shifts (each row of 16 by 1, 2, 4 and
@@ -257,9 +260,10 @@ __device__ __forceinline__ float candidate_logit(u64 c) {
 }
 __device__ __forceinline__ int candidate_place(u64 c) { return int(~uint32_t(c)); }
 
+template <bool VEC>
 __global__ void __launch_bounds__(kChunkThreads)
 sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
-                     double one, int vec) {
+                     double one) {
   constexpr int kParts = kChunkThreads / 64;
   __shared__ uint32_t count[kPlaces];
   __shared__ u64 mass[kPlaces];
@@ -269,7 +273,7 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int base = c * kChunk, len = min(kChunk, n - base);
   float v[kEach];
-  load_chunk(v, logits + size_t(row) * n + base, len, vec);
+  load_chunk<VEC>(v, logits + size_t(row) * n + base, len);
   const Row r(s, row, n, one);
   for (int i = tid; i < kPlaces; i += kChunkThreads) count[i] = 0, mass[i] = 0;
   fill_powers(powers);
@@ -345,6 +349,7 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   __shared__ int found[3];
   __shared__ double factor[kMaxChunks];
   __shared__ int shift[kMaxChunks];
+  __shared__ u64 sums[kMaxChunks];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Row r(s, row, n, one);
   const u64* tops = w.top + size_t(row) * chunks;
@@ -373,6 +378,7 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   for (int c = tid; c < chunks; c += kThreads) {
     const float t = candidate_logit(tops[c]);
     factor[c] = weight_of(t, top, r.inv, powers);
+    sums[c] = r.p < 1.0f ? rescale(w.mass[size_t(row) * chunks + c], factor[c]) : 0;
     shift[c] = t == top ? 0 : bin_below(tp, place(t, r.scale));
   }
   __syncthreads();
@@ -399,8 +405,10 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
       own_m += rescale(m[j], factor[min(c0 + j, chunks - 1)]);
     }
   }
-  if (by_mass)
-    for (int c = 0; c < chunks; ++c) all += rescale(w.mass[size_t(row) * chunks + c], factor[c]);
+  if (by_mass) {
+    for (int c = lane; c < chunks; c += 64) all += sums[c];
+    all = wave_sum(all);
+  }
   if (tid == kPlaces - 1) own_m = 0, own_n = 0;
   u64 cm = by_mass ? running(sh, own_m) : 0;
   uint32_t cn = by_count ? running(sh, own_n) : 0;
@@ -417,16 +425,18 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   // top-k's bin: the one in which the running count reaches k
   if (bn < uint32_t(r.k) && cn >= uint32_t(r.k)) found[0] = tid;
   __syncthreads();
+  // The last bin's weights are 0 (e^-31.97 of the largest is less than half of 2^-45), so nobody asks
+  // which of its tokens are kept, and a border there is none.
   int lo = 0x7fffffff, hi = -1, left = 0x7fffffff;
   if (r.least > 0.0) {
     // min-p's: one bin to either side of where its logit falls, for the roundings of the two
     const double at_least = top == INFINITY ? 0.0 : (double(top) + log(r.least) / r.inv) * r.scale;
     const double d = top == INFINITY ? 0.0 : tp - floor(at_least);
-    const int b = d < double(kPlaces - 1) ? int(fmax(d, 0.0)) : kPlaces - 1;
+    const int b = d < double(kPlaces - 2) ? int(fmax(d, 0.0)) : kPlaces - 2;
     lo = max(b - 1, 0);
-    hi = min(b + 1, kPlaces - 1);
+    hi = min(b + 1, kPlaces - 2);
   }
-  if (by_count) {
+  if (by_count && found[0] < kPlaces - 1) {
     const int b = found[0];
     if (b < lo) {
       lo = hi = b;
@@ -451,7 +461,7 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   o.outer_lo = outer ? lo : kPlaces;
   o.outer_hi = outer ? hi : kPlaces;
   o.inner_lo = r.p < 1.0f ? found[1] : kPlaces;
-  o.inner_hi = r.p < 1.0f ? (outer ? min(found[2], hi) : found[2]) : kPlaces;
+  o.inner_hi = r.p < 1.0f ? min(outer ? min(found[2], hi) : found[2], kPlaces - 2) : kPlaces;
   if (o.inner_lo > o.inner_hi) o.inner_lo = o.inner_hi;
   o.sure = min(o.outer_lo, o.inner_lo);
   o.sure_mass = o.sure ? mass[o.sure - 1] : 0;
@@ -464,9 +474,10 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   *st = o;
 }
 
+template <bool VEC>
 __global__ void __launch_bounds__(kChunkThreads)
 sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w, int n, int chunks,
-                      double one, int vec) {
+                      double one) {
   __shared__ double powers[64];
   __shared__ u64 red_m[kChunkThreads / 64];
   __shared__ int many, next;
@@ -488,7 +499,7 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
   }
   const int base = c * kChunk, len = min(kChunk, n - base);
   float v[kEach];
-  load_chunk(v, logits + size_t(row) * n + base, len, vec);
+  load_chunk<VEC>(v, logits + size_t(row) * n + base, len);
   fill_powers(powers);
   if (tid == 0) many = 0;
   __syncthreads();
@@ -838,12 +849,14 @@ extern "C" int ie_hip_sample_rows(int32_t* out, const float* logits, const float
   lay_out(&w, workspace, R, n);
   const Settings s{temperature, top_k, top_p, min_p, u};
   const double one = std::ldexp(1.0, weight_bits(n));
-  const int vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && n % 4 == 0;
+  const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && n % 4 == 0;
   const dim3 every(unsigned(R) * chunks), rows(R), wide(kChunkThreads), block(kThreads);
-  hipLaunchKernelGGL(sample_chunks_kernel, every, wide, 0, stream, logits, s, w, n, chunks, one, vec);
+  const auto each = vec ? sample_chunks_kernel<true> : sample_chunks_kernel<false>;
+  const auto collect = vec ? sample_collect_kernel<true> : sample_collect_kernel<false>;
+  hipLaunchKernelGGL(each, every, wide, 0, stream, logits, s, w, n, chunks, one);
   hipLaunchKernelGGL(sample_border_kernel, rows, block, 0, stream, out, s, w, n, chunks, one);
   if (top_k || top_p || min_p)
-    hipLaunchKernelGGL(sample_collect_kernel, every, wide, 0, stream, logits, s, w, n, chunks, one, vec);
+    hipLaunchKernelGGL(collect, every, wide, 0, stream, logits, s, w, n, chunks, one);
   hipLaunchKernelGGL(sample_draw_kernel, rows, block, 0, stream, out, logits, s, w, n, chunks, one);
   return check_launch("sample_rows");
 }

@@ -330,3 +330,22 @@ def test_two_captured_runs_in_turn(ie, dev):
             torch.cuda.synchronize()
             state[i] = r.check(*state[i])
             torch.randn(1000, device=dev).sum().item()
+
+
+@pytest.mark.parametrize("t", [0.02, 0.1, 0.3, 1.0, 4.0, 60.0])
+def test_sample_cold_hot_and_masked(ie, dev, t):
+    """Rows whose borders lie where weights vanish (cold), in one wide bin (hot), or past all that a
+    grammar leaves."""
+    rng = np.random.default_rng(int(t * 100))
+    R, n = 12, 60001
+    l = rows_of_logits(rng, R, n)
+    for r in range(0, R, 3):
+        l[r, rng.random(n) < 0.9995] = -np.inf
+    l[1] = -np.inf
+    l[1, 77] = -3
+    tt, u = np.full(R, t, np.float32), rng.random(R)
+    k = rng.integers(1, 400, R)
+    p, m = 0.5 + 0.5 * rng.random(R), 10.0 ** -rng.integers(1, 16, R)
+    for kk, pp, mm in ((k, None, None), (None, p, None), (None, None, m), (k, p, None), (k, None, m),
+                       (None, p, m), (k, p, m), (k * 100, p, m)):
+        assert draw(ie, dev, l, tt, u, kk, pp, mm).tolist() == expect(l, tt, u, kk, pp, mm)
