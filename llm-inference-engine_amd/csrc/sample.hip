@@ -9,8 +9,8 @@
 // What is kept is a prefix of the tokens ordered by (logit descending, index ascending). Four launches,
 // two over (row, chunk) that fill the chip and two over rows:
 //   chunks   the chunk's largest logit, its weight relative to that, and, for rows with a filter, a
-//            histogram of counts and weights over bins of T / 32 in the logit, which every chunk
-//            places alike (place())
+//            histogram of counts and weights over bins of T / 15.75 in the logit, which every
+//            chunk places alike (place())
 //   border   the row's histogram: which few bins hold the filters' borders; greedy rows end here
 //   collect  per chunk the weight of the bins above all borders; the tokens of the border bins go to
 //            the row's list
@@ -28,10 +28,10 @@ namespace iehip {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the launches over rows
-constexpr int kChunkThreads = 512, kEach = 16;           // of those over chunks, and logits of a thread
+constexpr int kChunkThreads = 512, kEach = 8;           // of those over chunks, and logits of a thread
 constexpr int kChunk = kChunkThreads * kEach;
-constexpr int kPlaces = 1024;              // bins of the rows' histograms, a thread each
-constexpr int kList = 4096;                // border tokens of a row
+constexpr int kPlaces = 512;               // bins of the rows' histograms, a thread each of `border`
+constexpr int kList = 6144;                // border tokens of a row
 constexpr int kDigits = 2048;
 constexpr int kMaxTokens = 1 << 22, kMaxChunks = kMaxTokens / kChunk;
 typedef unsigned long long u64;
@@ -53,8 +53,8 @@ struct RowState {
   int32_t sure, outer_lo, outer_hi, inner_lo, inner_hi;
   int32_t top_left;      // top-k: how many of the outer bins' tokens stay (INT_MAX: no limit)
   int32_t pad;
-  u64 sure_mass;         // of the bins below `sure`
   u64 outer_mass;        // of the bins below outer_lo
+  u64 outer_pass;        // of the outer bins' tokens that min-p keeps, where top-k does not bind
   u64 total;             // of the row
 };
 
@@ -101,7 +101,7 @@ struct Settings {
 
 // One row's settings, brought into their ranges.
 struct Row {
-  double inv, scale, least, one;  // 1 / T, bins per logit, min-p, the largest weight
+  double inv, rate, scale, least, one;  // 1 / T, weight_of's, bins per logit, min-p, the largest weight
   int k;                          // n: no top-k
   float p;                        // 1: no top-p
   bool greedy;
@@ -109,7 +109,8 @@ struct Row {
     const float t = s.temperature[row];
     greedy = !(t > 0.0f);
     inv = 1.0 / double(t);
-    scale = 32.0 * inv;
+    rate = 92.33248261689366 * inv;
+    scale = 15.75 * inv;
     const float m = s.min_p ? s.min_p[row] : 0.0f;
     least = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
     k = s.top_k ? s.top_k[row] : 0;
@@ -154,21 +155,19 @@ __device__ __forceinline__ void fill_powers(double* powers) {
   if (threadIdx.x < 64) powers[threadIdx.x] = kPowers[threadIdx.x];
 }
 
-// exp((l - top) / T) in [0, 1]. With m = round(64 x / ln 2) and r = x - m ln2 / 64, |r| <= 0.0055:
-// 2^(m div 64) 2^(m mod 64 / 64) (1 + r + .. + r^5 / 120), off by less than 2^-50 (r^6 / 720 =
-// 2^-54.5, and the roundings). 17 float64 instructions; the library's exp makes the first launch 64
-// rows x 151,936 half as long again.
-__device__ __forceinline__ double weight_of(float l, float top, double inv, const double* powers) {
-  if (l == top) return 1.0;
-  const double x = (double(l) - double(top)) * inv;
-  if (!(x > -45.0)) return 0.0;  // below 2^-64; l = -inf, top = inf
-  const double m = rint(x * 92.33248261689366);  // 64 / ln 2
-  double r = __builtin_fma(m, -0.010830424696249145, x);
-  r = __builtin_fma(m, -3.623510646634843e-19, r);  // ln2 / 64 less its leading 53 bits
-  double e = __builtin_fma(r, 1.0 / 120.0, 1.0 / 24.0);
-  e = __builtin_fma(e, r, 1.0 / 6.0);
-  e = __builtin_fma(e, r, 0.5);
-  e = __builtin_fma(e, r, 1.0);
+// exp((l - top) / T) in [0, 1]. With x = 64 (l - top) / (T ln 2), m = round(x) and r = x - m:
+// 2^(m div 64) 2^(m mod 64 / 64) (1 + c1 r + .. + c5 r^5), ck = (ln2 / 64)^k / k!. The series is off by
+// 2^-54.7, the product x by 2^-53 x, which is below 2^-53 of the largest weight where the weight is
+// e^x: 16 instructions, most of the launches over chunks (with the library's exp 64 rows x 151,936 took
+// half as long again). `rate` is 64 / (T ln 2).
+__device__ __forceinline__ double weight_of(float l, float top, double rate, const double* powers) {
+  const double d = double(l) - double(top);
+  const double x = fmax(d * rate, -64.0 * 64.0);  // 2^-64: nothing. l = -inf, and then T = inf, too
+  const double m = rint(x), r = x - m;
+  double e = __builtin_fma(r, 0x1.5d87fe78a6731p-40, 0x1.3b2ab6fba4e77p-31);
+  e = __builtin_fma(e, r, 0x1.c6b08d704a0c0p-23);
+  e = __builtin_fma(e, r, 0x1.ebfbdff82c58fp-15);
+  e = __builtin_fma(e, r, 0x1.62e42fefa39efp-7);
   e = __builtin_fma(e, r, 1.0);
   const int im = int(m);
   return ldexp(powers[im & 63] * e, im >> 6);
@@ -179,16 +178,18 @@ __device__ __forceinline__ u64 whole(double e, double one) {
   return static_cast<u64>(__double_as_longlong(__builtin_fma(e, one, 0x1p52))) & 0xFFFFFFFFFFFFFull;
 }
 
-// Where logits stand on the bins' axis: one function of l for every chunk.
-__device__ __forceinline__ double place(float l, double scale) {
-  return l == -INFINITY ? -INFINITY : floor(double(l) * scale);
-}
-__device__ __forceinline__ int bin_below(double top_place, double at) {
-  const double d = top_place - at;
-  return d < double(kPlaces - 1) ? int(d) : (top_place == at ? 0 : kPlaces - 1);
+// Where logits stand on the bins' axis, one function of l for every chunk, and how many bins below
+// another place that is (the last bin: that many or more).
+__device__ __forceinline__ double place(float l, double scale) { return floor(double(l) * scale); }
+__device__ __forceinline__ int bin_below(double top_place, float l, double scale) {
+  return int(fmin(top_place - place(l, scale), double(kPlaces - 1)));
 }
 
 __device__ __forceinline__ float read_logit(float v) { return v == v ? v : -INFINITY; }
+// In a row whose largest logit is +inf, as in one of zeros where it is and nothing elsewhere.
+__device__ __forceinline__ float in_row(float v, bool infinite) {
+  return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
+}
 
 // A thread's logits of a chunk: element e of vec4 u is number (u * kChunkThreads + tid) * 4 + e.
 __device__ __forceinline__ int chunk_index(int j) {
@@ -277,32 +278,37 @@ sample_chunks_kernel(const float* __restrict__ logits, Settings s, Workspace w, 
   const Row r(s, row, n, one);
   for (int i = tid; i < kPlaces; i += kChunkThreads) count[i] = 0, mass[i] = 0;
   fill_powers(powers);
-  u64 found = 0;
+  float most = v[0];
+  int where = 0;
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    const u64 c = candidate(v[j], base + chunk_index(j));
-    found = c > found ? c : found;
-  }
+  for (int j = 1; j < kEach; ++j)
+    if (v[j] > most) most = v[j], where = j;  // a thread's places rise with j
+  u64 found = candidate(most, base + chunk_index(where));
   found = wave_best(found);
   if (lane == 0) red_m[wave] = found;
   __syncthreads();
   found = 0;
 #pragma unroll
   for (int i = 0; i < kParts; ++i) found = red_m[i] > found ? red_m[i] : found;
-  const float best = candidate_logit(found);
+  float best = candidate_logit(found);
   const size_t rc = size_t(row) * chunks + c;
   if (tid == 0) w.top[rc] = found;
   const bool by_count = r.k < n, by_mass = r.p < 1.0f;
   if (r.greedy || (r.filtered(n) && !by_count && !by_mass)) return;  // min-p alone needs no sums here
+  if (best == INFINITY) {
+    best = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) v[j] = in_row(v[j], true);
+  }
   u64 sum = 0;
   const double tp = place(best, r.scale);
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     if (v[j] == -INFINITY) continue;  // (a masked row's tokens, and what is past the row)
-    const u64 m = by_count && !by_mass ? 0 : whole(weight_of(v[j], best, r.inv, powers), one);
+    const u64 m = by_count && !by_mass ? 0 : whole(weight_of(v[j], best, r.rate, powers), one);
     sum += m;
     if (!by_count && !by_mass) continue;
-    const int b = v[j] == best ? 0 : bin_below(tp, place(v[j], r.scale));
+    const int b = bin_below(tp, v[j], r.scale);
     if (b == kPlaces - 1) continue;  // what the others leave
     if (by_count) atomicAdd(&count[b], 1u);
     if (by_mass) atomicAdd(&mass[b], m);
@@ -328,24 +334,24 @@ __device__ __forceinline__ u64 rescale(u64 m, double factor) {
 }
 
 // Running sums over the workgroup's threads, own value included.
-template <class T>
-__device__ __forceinline__ T running(u64 (&sh)[kWaves], T x) {
+template <class T, int WAVES>
+__device__ __forceinline__ T running(u64 (&sh)[WAVES], T x) {
   const int wave = threadIdx.x >> 6;
   x = wave_running(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 63) sh[wave] = x;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) x += i < wave ? T(sh[i]) : T(0);
+  for (int i = 0; i < WAVES; ++i) x += i < wave ? T(sh[i]) : T(0);
   return x;
 }
 
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kPlaces)
 sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, int chunks, double one) {
   __shared__ uint32_t count[kPlaces];
   __shared__ u64 mass[kPlaces];
   __shared__ double powers[64];
-  __shared__ u64 sh[kWaves];
+  __shared__ u64 sh[kPlaces / 64];
   __shared__ int found[3];
   __shared__ double factor[kMaxChunks];
   __shared__ int shift[kMaxChunks];
@@ -356,30 +362,32 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   if (tid < 3) found[tid] = kPlaces - 1;
   fill_powers(powers);
   u64 best = 0;
-  for (int c = tid; c < chunks; c += kThreads) best = tops[c] > best ? tops[c] : best;
+  for (int c = tid; c < chunks; c += kPlaces) best = tops[c] > best ? tops[c] : best;
   best = wave_best(best);
   if (lane == 0) sh[wave] = best;
   __syncthreads();
   best = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) best = sh[i] > best ? sh[i] : best;
-  const float top = candidate_logit(best);
+  for (int i = 0; i < kPlaces / 64; ++i) best = sh[i] > best ? sh[i] : best;
+  const float largest = candidate_logit(best);
+  const bool infinite = largest == INFINITY;
+  const float top = infinite ? 0.0f : largest;
   RowState* st = w.rows + row;
   if (r.greedy || !best || !r.filtered(n)) {
     if (tid == 0) {
       const bool done = r.greedy || !best;
       st->mode = done ? kDone : kAll;
-      st->top = top;
+      st->top = largest;
       if (done) out[row] = best ? candidate_place(best) : 0;
     }
     return;
   }
   const double tp = place(top, r.scale);
-  for (int c = tid; c < chunks; c += kThreads) {
-    const float t = candidate_logit(tops[c]);
-    factor[c] = weight_of(t, top, r.inv, powers);
+  for (int c = tid; c < chunks; c += kPlaces) {
+    const float t = in_row(candidate_logit(tops[c]), infinite);
+    factor[c] = weight_of(t, top, r.rate, powers);
     sums[c] = r.p < 1.0f ? rescale(w.mass[size_t(row) * chunks + c], factor[c]) : 0;
-    shift[c] = t == top ? 0 : bin_below(tp, place(t, r.scale));
+    shift[c] = t > -INFINITY ? bin_below(tp, t, r.scale) : kPlaces;
   }
   __syncthreads();
   // This thread's bin over the chunks: each has it further down by how far its own top is below the
@@ -430,8 +438,7 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   int lo = 0x7fffffff, hi = -1, left = 0x7fffffff;
   if (r.least > 0.0) {
     // min-p's: one bin to either side of where its logit falls, for the roundings of the two
-    const double at_least = top == INFINITY ? 0.0 : (double(top) + log(r.least) / r.inv) * r.scale;
-    const double d = top == INFINITY ? 0.0 : tp - floor(at_least);
+    const double d = tp - floor((double(top) + log(r.least) / r.inv) * r.scale);
     const int b = d < double(kPlaces - 2) ? int(fmax(d, 0.0)) : kPlaces - 2;
     lo = max(b - 1, 0);
     hi = min(b + 1, kPlaces - 2);
@@ -457,15 +464,15 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   __syncthreads();
   if (tid != 0) return;
   RowState o;
-  o.top = top;
+  o.top = largest;
   o.outer_lo = outer ? lo : kPlaces;
   o.outer_hi = outer ? hi : kPlaces;
   o.inner_lo = r.p < 1.0f ? found[1] : kPlaces;
   o.inner_hi = r.p < 1.0f ? min(outer ? min(found[2], hi) : found[2], kPlaces - 2) : kPlaces;
   if (o.inner_lo > o.inner_hi) o.inner_lo = o.inner_hi;
   o.sure = min(o.outer_lo, o.inner_lo);
-  o.sure_mass = o.sure ? mass[o.sure - 1] : 0;
   o.outer_mass = below;
+  o.outer_pass = 0;
   o.total = total;
   o.top_left = left;
   o.pad = 0;
@@ -488,10 +495,11 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
   const size_t rc = size_t(row) * chunks + c;
   const int sure = st->sure, outer_lo = st->outer_lo, outer_hi = st->outer_hi;
   const int inner_lo = st->inner_lo, inner_hi = st->inner_hi;
-  const float top = st->top, chunk_top = candidate_logit(w.top[rc]);
+  const bool infinite = st->top == INFINITY;
+  const float top = infinite ? 0.0f : st->top, chunk_top = in_row(candidate_logit(w.top[rc]), infinite);
   const Row r(s, row, n, one);
   const double tp = place(top, r.scale);
-  const int nearest = chunk_top == top ? 0 : bin_below(tp, place(chunk_top, r.scale));
+  const int nearest = chunk_top > -INFINITY ? bin_below(tp, chunk_top, r.scale) : kPlaces;
   const int last = max(sure - 1, max(outer_hi < kPlaces ? outer_hi : -1, inner_hi < kPlaces ? inner_hi : -1));
   if (nearest > last) {
     if (tid == 0) w.mass[rc] = 0;
@@ -503,19 +511,35 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
   fill_powers(powers);
   if (tid == 0) many = 0;
   __syncthreads();
-  u64 sum = 0;
+  // Where top-k does not bind, min-p decides its bins' tokens one by one, and only top-p's are listed.
+  const bool free = st->top_left == 0x7fffffff;
+  u64 sum = 0, pass = 0;
   uint32_t listed = 0;  // a bit per logit
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
-    if (chunk_index(j) >= len) continue;
-    const int b = v[j] == top ? 0 : bin_below(tp, place(v[j], r.scale));
-    if (b < sure)
-      sum += whole(weight_of(v[j], top, r.inv, powers), one);
-    else if ((b >= outer_lo && b <= outer_hi) || (b >= inner_lo && b <= inner_hi))
+    v[j] = in_row(v[j], infinite);
+    if (v[j] == -INFINITY) continue;
+    const int b = bin_below(tp, v[j], r.scale);
+    const bool outer = b >= outer_lo && b <= outer_hi, inner = b >= inner_lo && b <= inner_hi;
+    if (b < sure || (outer && free)) {
+      const double x = weight_of(v[j], top, r.rate, powers);
+      if (b >= sure && x < r.least) continue;
+      const u64 m = whole(x, one);
+      if (outer) pass += m;
+      if (inner)
+        listed |= 1u << j;
+      else if (b < inner_lo)
+        sum += m;
+    } else if (outer || inner) {
       listed |= 1u << j;
+    }
   }
   sum = wave_sum(sum);
   if (lane == 0) red_m[wave] = sum;
+  if (free && r.p < 1.0f) {
+    pass = wave_sum(pass);
+    if (lane == 0 && pass) atomicAdd(&st->outer_pass, pass);
+  }
   int at = listed ? atomicAdd(&many, __popc(listed)) : 0;
   __syncthreads();
   if (tid == 0) {
@@ -601,11 +625,13 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   const float* l = logits + size_t(row) * n;
   const Row r(s, row, n, one);
   const bool filtered = st.mode != kAll, all = filtered && st.listed > kList;
+  const bool infinite = st.top == INFINITY;
+  if (infinite) st.top = 0.0f;
   const double tp = place(st.top, r.scale);
   fill_powers(powers);
   if (all) {
     st.sure = 0, st.outer_lo = 0, st.outer_hi = kPlaces - 1, st.inner_lo = 0, st.inner_hi = kPlaces - 1;
-    st.sure_mass = st.outer_mass = 0;
+    st.outer_mass = 0;
     st.top_left = r.k < n ? r.k : 0x7fffffff;
   }
   const int items = !filtered ? 0 : all ? n : st.listed;
@@ -631,9 +657,9 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
     digits = any >> 21 ? 3 : any >> 10 ? 2 : 1;
     common_prefix = digits == 3 ? 0 : digits == 2 ? o >> 21 : o >> 10;
   }
-  auto entry = [&](int i) { return all ? Entry{read_logit(l[i]), i} : list[i]; };
-  auto bin_of = [&](float v) { return v == st.top ? 0 : bin_below(tp, place(v, r.scale)); };
-  auto weight = [&](float v) { return weight_of(v, st.top, r.inv, powers); };
+  auto entry = [&](int i) { return all ? Entry{in_row(read_logit(l[i]), infinite), i} : list[i]; };
+  auto bin_of = [&](float v) { return v > -INFINITY ? bin_below(tp, v, r.scale) : kPlaces - 1; };
+  auto weight = [&](float v) { return weight_of(v, st.top, r.rate, powers); };
 
   // The kept part of the list: at or above (key, last index), in order, of bins up to `end`, with the
   // least weight where the bin is one of the outer ones.
@@ -701,7 +727,9 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   }
   if (filtered && r.p < 1.0f) {
     u64 of = st.total;
-    if (st.outer_lo < kPlaces) {
+    if (st.outer_lo < kPlaces && !all && st.top_left == 0x7fffffff) {
+      of = st.outer_mass + st.outer_pass;
+    } else if (st.outer_lo < kPlaces) {
       u64 m = 0;
       for (int i = tid; i < items; i += kThreads) {
         const Entry e = entry(i);
@@ -718,6 +746,10 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
       for (int i = 0; i < kWaves; ++i) of += red_m[i];
     }
     const double goal = double(r.p) * double(of);
+    // What the list's tokens come on top of: the chunks' sums so far.
+    u64 base = 0;
+    for (int i = lane; i < chunks; i += 64) base += chunk_mass[i];
+    base = wave_sum(base);
     end = st.inner_hi;
     select(
         std::true_type{},
@@ -727,11 +759,11 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
           m = whole(x, one);
           return stays(v, i, b, x);
         },
-        [&](u64 m) { return double(st.sure_mass + m) >= goal; },
+        [&](u64 m) { return double(base + m) >= goal; },
         [&](uint32_t equal, u64 m, uint32_t o) {
           const float v = __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
           const double each = double(whole(weight(v), one));
-          const double need = (goal - double(st.sure_mass + m)) / each;
+          const double need = (goal - double(base + m)) / each;
           return need <= 1.0 ? 1u : uint32_t(fmin(ceil(need), double(equal)));
         });
   }
@@ -739,7 +771,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   if (!filtered) {
     for (int i = tid; i < chunks; i += kThreads) {
       const size_t rc = size_t(row) * chunks + i;
-      chunk_mass[i] = rescale(w.mass[rc], weight(candidate_logit(w.top[rc])));
+      chunk_mass[i] = rescale(w.mass[rc], weight(in_row(candidate_logit(w.top[rc]), infinite)));
     }
   }
   auto kept = [&](float v, int i) -> u64 {
@@ -781,7 +813,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   u64 want = need - before_of;
   if (!filtered) {  // in the chunk's own units, whose sum is at hand
     const size_t rc = size_t(row) * chunks + chosen;
-    const float chunk_top = candidate_logit(w.top[rc]);
+    const float chunk_top = in_row(candidate_logit(w.top[rc]), infinite);
     if (chunk_top != st.top) {
       const double f = weight(chunk_top);
       want = max(u64(1), min(w.mass[rc], static_cast<u64>(ceil(double(want) / f))));
@@ -793,7 +825,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   const int lo = wave * kPart * 64 + lane;
   float v[kPart];
 #pragma unroll
-  for (int j = 0; j < kPart; ++j) v[j] = lo + 64 * j < len ? read_logit(l[base + lo + 64 * j]) : -INFINITY;
+  for (int j = 0; j < kPart; ++j) v[j] = in_row(lo + 64 * j < len ? read_logit(l[base + min(lo + 64 * j, len - 1)]) : -INFINITY, infinite);
   u64 p[kPart], m = 0;
 #pragma unroll
   for (int j = 0; j < kPart; ++j) {
@@ -854,7 +886,7 @@ extern "C" int ie_hip_sample_rows(int32_t* out, const float* logits, const float
   const auto each = vec ? sample_chunks_kernel<true> : sample_chunks_kernel<false>;
   const auto collect = vec ? sample_collect_kernel<true> : sample_collect_kernel<false>;
   hipLaunchKernelGGL(each, every, wide, 0, stream, logits, s, w, n, chunks, one);
-  hipLaunchKernelGGL(sample_border_kernel, rows, block, 0, stream, out, s, w, n, chunks, one);
+  hipLaunchKernelGGL(sample_border_kernel, rows, dim3(kPlaces), 0, stream, out, s, w, n, chunks, one);
   if (top_k || top_p || min_p)
     hipLaunchKernelGGL(collect, every, wide, 0, stream, logits, s, w, n, chunks, one);
   hipLaunchKernelGGL(sample_draw_kernel, rows, block, 0, stream, out, logits, s, w, n, chunks, one);

@@ -349,3 +349,16 @@ def test_sample_cold_hot_and_masked(ie, dev, t):
     for kk, pp, mm in ((k, None, None), (None, p, None), (None, None, m), (k, p, None), (k, None, m),
                        (None, p, m), (k, p, m), (k * 100, p, m)):
         assert draw(ie, dev, l, tt, u, kk, pp, mm).tolist() == expect(l, tt, u, kk, pp, mm)
+
+
+def test_sample_wide_borders(ie, dev):
+    """min-p and top-k borders in the thick of a row, among more tokens than a few bins are listed for,
+    alone and under top-p."""
+    rng = np.random.default_rng(77)
+    R, n = 8, 151936
+    l = (rng.standard_normal((R, n)) * 2.5).astype(np.float32)
+    l[::2] = np.round(l[::2] * 4) / 4  # few values, thousands of tokens each
+    t, u = np.full(R, 1.5, np.float32), rng.random(R)
+    m, p, k = 10.0 ** -rng.uniform(1, 5, R), 0.3 + 0.69 * rng.random(R), rng.integers(2000, 140000, R)
+    for kk, pp, mm in ((None, None, m), (None, p, m), (k, None, None), (k, p, None), (k, p, m), (None, p, None)):
+        assert draw(ie, dev, l, t, u, kk, pp, mm).tolist() == expect(l, t, u, kk, pp, mm)
