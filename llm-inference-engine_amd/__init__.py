@@ -15,6 +15,7 @@ The package directory name is not an identifier; load it with ``load()`` from
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -461,33 +462,44 @@ def _tensor(t, name: str, dtype, shape, like=None):
     """Refuses a tensor the kernels would read wrongly: another type or shape, elements that do
     not follow each other, another device than `like` (the call's first tensor) or, for that
     one, than the current device, whose stream the launch goes to."""
-    import torch
     if t.dtype != dtype:
         raise IeHipError(EINVAL, f"{name}: expected {dtype}, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise IeHipError(EINVAL, f"{name}: expected shape {tuple(shape)}, not {tuple(t.shape)}")
     if not t.is_contiguous():
         raise IeHipError(EINVAL, f"{name}: must be contiguous")
+    device = t.get_device()
     if like is not None:
-        if t.device != like.device:
+        if device != like.get_device():
             raise IeHipError(EINVAL, f"{name}: on {t.device}, not on {like.device}")
-    elif not t.is_cuda or t.device.index != torch.cuda.current_device():
+    elif device < 0 or device != _current_device():
         raise IeHipError(EINVAL, f"{name}: on {t.device}, not on the current GPU")
 
 
-def _tokens(x, cols: int, name: str) -> int:
-    """Rows of the activations x [..., cols]; checks x as _tensor does."""
+def _current_device() -> int:
     import torch
-    _tensor(x, f"{name}: x", torch.float32, None)
+    return torch._C._cuda_getDevice()
+
+
+def _f32():
+    import torch
+    return torch.float32
+
+
+def _tokens(x, w: "MatrixQ4", name: str) -> int:
+    """Rows of the activations x [..., w.cols]; checks x as _tensor does."""
+    _tensor(x, f"{name}: x", _f32(), None)
+    cols = w.cols
     if x.dim() == 0 or x.shape[-1] != cols:
         raise IeHipError(EINVAL, f"{name}: x must have {cols} columns")
+    if w.device != x.get_device():
+        raise IeHipError(EINVAL, f"{name}: the weights are not on {x.device}")
     return x.numel() // cols
 
 
 def _rows_of(t, rows: int, cols: int, name: str, like) -> None:
     """t holds `rows` rows of `cols` f32 values."""
-    import torch
-    _tensor(t, name, torch.float32, None, like)
+    _tensor(t, name, _f32(), None, like)
     if t.dim() == 0 or t.shape[-1] != cols or t.numel() != rows * cols:
         raise IeHipError(EINVAL, f"{name}: expected {rows} rows of {cols}, not {tuple(t.shape)}")
 
@@ -498,7 +510,7 @@ def _workspace(workspace, need: int, name: str, like):
         return None
     if workspace is None:
         raise IeHipError(EINVAL, f"{name}: needs a workspace of {need} bytes")
-    if workspace.device != like.device:
+    if workspace.get_device() != like.get_device():
         raise IeHipError(EINVAL, f"{name}: workspace on {workspace.device}, not on {like.device}")
     if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
         raise IeHipError(EINVAL, f"{name}: needs a contiguous workspace of {need} bytes")
@@ -524,7 +536,7 @@ def matrix_q4(data, scale, group: int, zero=None) -> MatrixQ4:
         _tensor(zero, "matrix_q4: zero", torch.uint8, shape, data)
     m = MatrixQ4(data.data_ptr(), scale.data_ptr(), None if zero is None else zero.data_ptr(),
                  kinds[scale.dtype], group, rows, cols)
-    m.tensors = (data, scale, zero)
+    m.tensors, m.device = (data, scale, zero), data.get_device()
     return m
 
 
@@ -535,15 +547,19 @@ def matmul_q4_workspace(T: int, cols: int, device="cuda"):
     return torch.empty(max(n, 256), dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=4096)
+def _q4_need(T: int, cols: int) -> int:
+    return int(lib().ie_hip_matmul_q4_workspace_bytes(T, cols))
+
+
 def _q4_workspace(workspace, T: int, w: MatrixQ4, name: str, like):
-    need = int(lib().ie_hip_matmul_q4_workspace_bytes(T, w.cols))
-    return _workspace(workspace, need, name, like)
+    return _workspace(workspace, _q4_need(T, w.cols), name, like)
 
 
 def matmul_q4(y, x, w: MatrixQ4, bias=None, accumulate: bool = False, workspace=None,
               stream=None) -> None:
     """matmul() over a 4-bit matrix: y (+)= x . W^T + bias (no reference counterpart)."""
-    T = _tokens(x, w.cols, "matmul_q4")
+    T = _tokens(x, w, "matmul_q4")
     _rows_of(y, T, w.rows, "matmul_q4: y", x)
     if bias is not None:
         _rows_of(bias, 1, w.rows, "matmul_q4: bias", x)
@@ -553,7 +569,7 @@ def matmul_q4(y, x, w: MatrixQ4, bias=None, accumulate: bool = False, workspace=
 
 def qkv_proj_q4(q, k, v, x, w_qkv: MatrixQ4, b_qkv=None, workspace=None, stream=None) -> None:
     """qkv_proj() over a 4-bit matrix (no reference counterpart)."""
-    T = _tokens(x, w_qkv.cols, "qkv_proj_q4")
+    T = _tokens(x, w_qkv, "qkv_proj_q4")
     q_dim, kv_dim = q.shape[-1], k.shape[-1]
     _rows_of(q, T, q_dim, "qkv_proj_q4: q", x)
     _rows_of(k, T, kv_dim, "qkv_proj_q4: k", x)
@@ -567,7 +583,9 @@ def qkv_proj_q4(q, k, v, x, w_qkv: MatrixQ4, b_qkv=None, workspace=None, stream=
 
 def gate_up_silu_q4(out, x, w_gate: MatrixQ4, w_up: MatrixQ4, workspace=None, stream=None) -> None:
     """gate_up_silu() over two 4-bit matrices (no reference counterpart)."""
-    T = _tokens(x, w_gate.cols, "gate_up_silu_q4")
+    T = _tokens(x, w_gate, "gate_up_silu_q4")
+    if w_up.device != w_gate.device:
+        raise IeHipError(EINVAL, "gate_up_silu_q4: gate and up on two devices")
     _rows_of(out, T, w_gate.rows, "gate_up_silu_q4: out", x)
     ws = _q4_workspace(workspace, T, w_gate, "gate_up_silu_q4", x)
     _check(_native().ie_hip_gate_up_silu_q4(out, x, w_gate, w_up, T, ws, _stream(stream)))
@@ -639,7 +657,7 @@ def adjust_logits(out, logits, rules: LogitRules, stream=None) -> None:
         raise IeHipError(EINVAL, f"adjust_logits: rules of {rules.rows} rows for {R}")
     if rules.words is not None and rules.words != -(-n // 32):
         raise IeHipError(EINVAL, f"adjust_logits: a mask of {rules.words} words for {n} tokens")
-    if rules.tensors and rules.tensors[0].device != logits.device:
+    if rules.tensors and rules.tensors[0].get_device() != logits.get_device():
         raise IeHipError(EINVAL, f"adjust_logits: rules on {rules.tensors[0].device}")
     _check(_native().ie_hip_adjust_logits(out, logits, rules, R, n, _stream(stream)))
 
@@ -649,6 +667,11 @@ def sample_rows_workspace(R: int, n: int, device="cuda"):
     import torch
     b = int(lib().ie_hip_sample_rows_workspace_bytes(R, n))
     return torch.empty(max(b, 256), dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _sample_need(R: int, n: int) -> int:
+    return int(lib().ie_hip_sample_rows_workspace_bytes(R, n))
 
 
 def sample_rows(out, logits, temperature, u, top_k=None, top_p=None, min_p=None, workspace=None,
@@ -665,8 +688,7 @@ def sample_rows(out, logits, temperature, u, top_k=None, top_p=None, min_p=None,
                            ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
         if t is not None:
             _tensor(t, f"sample_rows: {name}", dtype, (R,), logits)
-    need = int(lib().ie_hip_sample_rows_workspace_bytes(R, n))
-    ws = _workspace(workspace, need, "sample_rows", logits)
+    ws = _workspace(workspace, _sample_need(R, n), "sample_rows", logits)
     _check(_native().ie_hip_sample_rows(out, logits, temperature, top_k, top_p, min_p, u, R, n, ws,
                                         _stream(stream)))
 

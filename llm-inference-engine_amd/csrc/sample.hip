@@ -395,24 +395,24 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   const bool by_count = r.k < n, by_mass = r.p < 1.0f;
   u64 own_m = 0, all = 0;
   uint32_t own_n = 0;
-  constexpr int kBatch = 8;
-  for (int c0 = 0; c0 < chunks; c0 += kBatch) {
-    uint32_t cc[kBatch];
-    u64 m[kBatch];
+  constexpr int kBatch = 20;  // loads under way at once
+  auto gather = [&](const auto* bins, const auto& add) {
+    for (int c0 = 0; c0 < chunks; c0 += kBatch) {
+      std::decay_t<decltype(*bins)> got[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int c = min(c0 + j, chunks - 1), bin = tid - shift[c];
-      const bool in = c0 + j < chunks && bin >= 0;
-      const size_t at = (size_t(row) * chunks + c) * kPlaces + (in ? bin : 0);
-      cc[j] = in && by_count ? w.bin_count[at] : 0;
-      m[j] = in && by_mass ? w.bin_mass[at] : 0;
-    }
+      for (int j = 0; j < kBatch; ++j) {
+        const int c = min(c0 + j, chunks - 1);
+        got[j] = bins[(size_t(row) * chunks + c) * kPlaces + max(tid - shift[c], 0)];
+      }
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      own_n += cc[j];
-      own_m += rescale(m[j], factor[min(c0 + j, chunks - 1)]);
+      for (int j = 0; j < kBatch; ++j) {
+        const int c = min(c0 + j, chunks - 1);
+        if (c0 + j < chunks && tid >= shift[c]) add(got[j], c);
+      }
     }
-  }
+  };
+  if (by_mass) gather(w.bin_mass, [&](u64 m, int c) { own_m += rescale(m, factor[c]); });
+  if (by_count) gather(w.bin_count, [&](uint32_t c, int) { own_n += c; });
   if (by_mass) {
     for (int c = lane; c < chunks; c += 64) all += sums[c];
     all = wave_sum(all);
