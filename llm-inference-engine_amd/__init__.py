@@ -476,9 +476,16 @@ def _tensor(t, name: str, dtype, shape, like=None):
         raise IeHipError(EINVAL, f"{name}: on {t.device}, not on the current GPU")
 
 
+_get_device = None
+
+
 def _current_device() -> int:
-    import torch
-    return torch._C._cuda_getDevice()
+    global _get_device
+    if _get_device is None:
+        import torch
+        torch.cuda.current_device()  # initialises the device
+        _get_device = torch._C._cuda_getDevice
+    return _get_device()
 
 
 def _f32():
@@ -488,19 +495,20 @@ def _f32():
 
 def _tokens(x, w: "MatrixQ4", name: str) -> int:
     """Rows of the activations x [..., w.cols]; checks x as _tensor does."""
-    _tensor(x, f"{name}: x", _f32(), None)
-    cols = w.cols
-    if x.dim() == 0 or x.shape[-1] != cols:
-        raise IeHipError(EINVAL, f"{name}: x must have {cols} columns")
-    if w.device != x.get_device():
+    cols, device = w.cols, w.device
+    T = x.numel() // cols
+    if not (device >= 0 and _native().fits(x, T * cols, cols, device) and device == _current_device()):
+        _tensor(x, f"{name}: x", _f32(), None)
+        if x.dim() == 0 or x.shape[-1] != cols:
+            raise IeHipError(EINVAL, f"{name}: x must have {cols} columns")
         raise IeHipError(EINVAL, f"{name}: the weights are not on {x.device}")
-    return x.numel() // cols
+    return T
 
 
-def _rows_of(t, rows: int, cols: int, name: str, like) -> None:
-    """t holds `rows` rows of `cols` f32 values."""
-    _tensor(t, name, _f32(), None, like)
-    if t.dim() == 0 or t.shape[-1] != cols or t.numel() != rows * cols:
+def _rows_of(t, rows: int, cols: int, name: str, like, device: int) -> None:
+    """t holds `rows` rows of `cols` f32 values on `device`, which is like's."""
+    if not _native().fits(t, rows * cols, cols, device):
+        _tensor(t, name, _f32(), None, like)
         raise IeHipError(EINVAL, f"{name}: expected {rows} rows of {cols}, not {tuple(t.shape)}")
 
 
@@ -560,9 +568,9 @@ def matmul_q4(y, x, w: MatrixQ4, bias=None, accumulate: bool = False, workspace=
               stream=None) -> None:
     """matmul() over a 4-bit matrix: y (+)= x . W^T + bias (no reference counterpart)."""
     T = _tokens(x, w, "matmul_q4")
-    _rows_of(y, T, w.rows, "matmul_q4: y", x)
+    _rows_of(y, T, w.rows, "matmul_q4: y", x, w.device)
     if bias is not None:
-        _rows_of(bias, 1, w.rows, "matmul_q4: bias", x)
+        _rows_of(bias, 1, w.rows, "matmul_q4: bias", x, w.device)
     ws = _q4_workspace(workspace, T, w, "matmul_q4", x)
     _check(_native().ie_hip_matmul_q4(y, x, w, bias, T, int(accumulate), ws, _stream(stream)))
 
@@ -571,11 +579,11 @@ def qkv_proj_q4(q, k, v, x, w_qkv: MatrixQ4, b_qkv=None, workspace=None, stream=
     """qkv_proj() over a 4-bit matrix (no reference counterpart)."""
     T = _tokens(x, w_qkv, "qkv_proj_q4")
     q_dim, kv_dim = q.shape[-1], k.shape[-1]
-    _rows_of(q, T, q_dim, "qkv_proj_q4: q", x)
-    _rows_of(k, T, kv_dim, "qkv_proj_q4: k", x)
-    _rows_of(v, T, kv_dim, "qkv_proj_q4: v", x)
+    _rows_of(q, T, q_dim, "qkv_proj_q4: q", x, w_qkv.device)
+    _rows_of(k, T, kv_dim, "qkv_proj_q4: k", x, w_qkv.device)
+    _rows_of(v, T, kv_dim, "qkv_proj_q4: v", x, w_qkv.device)
     if b_qkv is not None:
-        _rows_of(b_qkv, 1, w_qkv.rows, "qkv_proj_q4: bias", x)
+        _rows_of(b_qkv, 1, w_qkv.rows, "qkv_proj_q4: bias", x, w_qkv.device)
     ws = _q4_workspace(workspace, T, w_qkv, "qkv_proj_q4", x)
     _check(_native().ie_hip_qkv_proj_q4(q, k, v, x, w_qkv, b_qkv, T, q_dim, kv_dim, ws,
                                         _stream(stream)))
@@ -586,7 +594,7 @@ def gate_up_silu_q4(out, x, w_gate: MatrixQ4, w_up: MatrixQ4, workspace=None, st
     T = _tokens(x, w_gate, "gate_up_silu_q4")
     if w_up.device != w_gate.device:
         raise IeHipError(EINVAL, "gate_up_silu_q4: gate and up on two devices")
-    _rows_of(out, T, w_gate.rows, "gate_up_silu_q4: out", x)
+    _rows_of(out, T, w_gate.rows, "gate_up_silu_q4: out", x, w_gate.device)
     ws = _q4_workspace(workspace, T, w_gate, "gate_up_silu_q4", x)
     _check(_native().ie_hip_gate_up_silu_q4(out, x, w_gate, w_up, T, ws, _stream(stream)))
 

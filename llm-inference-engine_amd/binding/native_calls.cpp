@@ -33,7 +33,8 @@ constexpr int kStruct<ie_matrix_q4> = 1;
 template <>
 constexpr int kStruct<ie_logit_rules> = 2;
 constexpr const char* kStructNames[3] = {"Matrix", "MatrixQ4", "LogitRules"};
-PyObject *g_data_ptr = nullptr, *g_numel = nullptr, *g_dtype = nullptr;
+PyObject *g_data_ptr = nullptr, *g_numel = nullptr, *g_dtype = nullptr, *g_get_device = nullptr,
+         *g_is_contiguous = nullptr, *g_dim = nullptr, *g_size = nullptr, *g_minus_one = nullptr;
 
 bool as_u64(PyObject* o, unsigned long long* v) {
   if (!PyLong_Check(o)) {
@@ -197,11 +198,51 @@ PyObject* set_types(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// fits(t, numel, last, device): whether t is a contiguous float32 tensor of that many elements, that
+// last dimension and that device (a tensor's checks in Python cost three times as much).
+PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "expected a tensor, its elements, last dimension and device");
+    return nullptr;
+  }
+  PyObject* dtype = PyObject_GetAttr(args[0], g_dtype);
+  if (!dtype) return nullptr;
+  const bool f32 = dtype == g_dtypes[0];
+  Py_DECREF(dtype);
+  if (!f32) Py_RETURN_FALSE;
+  // The three answers, each compared as an object: numel(), get_device(), is_contiguous().
+  PyObject* const methods[3] = {g_numel, g_get_device, g_is_contiguous};
+  PyObject* const wanted[3] = {args[1], args[3], Py_True};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* r = PyObject_CallMethodNoArgs(args[0], methods[i]);
+    if (!r) return nullptr;
+    const int same = PyObject_RichCompareBool(r, wanted[i], Py_EQ);
+    Py_DECREF(r);
+    if (same < 0) return nullptr;
+    if (!same) Py_RETURN_FALSE;
+  }
+  PyObject* dims = PyObject_CallMethodNoArgs(args[0], g_dim);
+  if (!dims) return nullptr;
+  const long d = PyLong_AsLong(dims);
+  Py_DECREF(dims);
+  if (d < 1) {
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_FALSE;
+  }
+  PyObject* size = PyObject_CallMethodOneArg(args[0], g_size, g_minus_one);
+  if (!size) return nullptr;
+  const int same = PyObject_RichCompareBool(size, args[2], Py_EQ);
+  Py_DECREF(size);
+  if (same < 0) return nullptr;
+  return PyBool_FromLong(same);
+}
+
 #define IE_CALL(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&call<&name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     {"set_types", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&set_types)), METH_FASTCALL,
      nullptr},
+    {"fits", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&fits)), METH_FASTCALL, nullptr},
     IE_CALL(ie_hip_rope_and_cache),
     IE_CALL(ie_hip_attention),
     IE_CALL(ie_hip_attention_noalloc),
@@ -232,7 +273,15 @@ int exec(PyObject*) {
   if (!g_data_ptr) g_data_ptr = PyUnicode_InternFromString("data_ptr");
   if (!g_numel) g_numel = PyUnicode_InternFromString("numel");
   if (!g_dtype) g_dtype = PyUnicode_InternFromString("dtype");
-  return g_data_ptr && g_numel && g_dtype ? 0 : -1;
+  if (!g_get_device) g_get_device = PyUnicode_InternFromString("get_device");
+  if (!g_is_contiguous) g_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+  if (!g_dim) g_dim = PyUnicode_InternFromString("dim");
+  if (!g_size) g_size = PyUnicode_InternFromString("size");
+  if (!g_minus_one) g_minus_one = PyLong_FromLong(-1);
+  return g_data_ptr && g_numel && g_dtype && g_get_device && g_is_contiguous && g_dim && g_size &&
+                 g_minus_one
+             ? 0
+             : -1;
 }
 
 PyModuleDef_Slot slots[] = {{Py_mod_exec, reinterpret_cast<void*>(&exec)}, {0, nullptr}};

@@ -369,8 +369,21 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
       }
     }
   };
+  // Two stages ahead of what is multiplied.
+  int ahead_tile = first, ahead_b = b0;
+  auto issue_next = [&](int stage) {
+    if (ahead_tile >= row_tiles || b0 >= b1) return false;
+    issue(ahead_tile, ahead_b, stage);
+    ahead_b += SB;
+    if (ahead_b >= b1) {
+      ahead_b = b0;
+      ahead_tile += hop;
+    }
+    return true;
+  };
+  issue_next(0);
+  bool more = issue_next(1);  // whether the stage after the one at hand is under way
   int stage = 0;
-  if (first < row_tiles && b0 < b1) issue(first, b0, 0);
   for (int u = threadIdx.x >> 4; u < blocks * T; u += 32) {
     const int b = u / T, tok = u - b * T, k8 = r, k = b * kBlock + 8 * k8;
     float v[8];
@@ -389,19 +402,12 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
     for (int n = 0; n < NA; ++n) total[n] = acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     int slot = 0;
     for (int b = b0; b < b1; b += SB) {
-      wait_lds();  // the other stage has been read
-      if (b + SB < b1) {
-        issue(tile, b + SB, stage ^ 1);
+      if (more)
         wait_vmcnt<F::kLoads>();
-      } else if (tile + hop < row_tiles) {
-        issue(tile + hop, b0, stage ^ 1);
-        wait_vmcnt<F::kLoads>();
-      } else {
+      else
         wait_vmcnt<0>();
-      }
       asm volatile("" ::: "memory");
       const unsigned char* from = ring + stage * F::kStage;
-      stage ^= 1;
 #pragma unroll
       for (int sb = 0; sb < SB; ++sb) {
         if (b + sb >= b1) break;
@@ -444,6 +450,9 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
             ++slot;
           }
       }
+      wait_lds();  // the stage has been read
+      more = issue_next(stage);
+      stage ^= 1;
     }
     if constexpr (SPLIT) {
       f32x4* sums = reinterpret_cast<f32x4*>(dyn + F::kSums);

@@ -127,3 +127,15 @@ def test_native_calls_take_their_own_structure(ie):
         calls.ie_hip_adjust_logits(z(1, 8), z(1, 8), m, 0, 8, 0)
     with pytest.raises(TypeError, match="Matrix"):
         calls.ie_hip_matmul(z(1, 16), z(1, 64), q4(ie), None, 0, 0, 0)
+
+
+def test_fits(ie):
+    fits, z = ie._native().fits, torch.zeros
+    assert fits(z(2, 3), 6, 3, -1) and fits(z(0, 3), 0, 3, -1)
+    for t, n, last, dev in ((z(2, 3), 6, 2, -1), (z(2, 3), 5, 3, -1), (z(2, 3), 6, 3, 0), (z(()), 1, 1, -1),
+                            (z(2, 3, dtype=torch.float64), 6, 3, -1), (z(3, 2).t(), 6, 3, -1)):
+        assert not fits(t, n, last, dev)
+    with pytest.raises(AttributeError):
+        fits(5, 1, 1, 0)
+    with pytest.raises(TypeError):
+        fits(z(1), 1, 1)
