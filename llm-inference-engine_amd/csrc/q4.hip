@@ -369,7 +369,10 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
       }
     }
   };
-  // Two stages ahead of what is multiplied.
+  // One block a stage, which is a slot's whole share: two stages go out before the activations are split.
+  // More blocks: the next stage goes out before a stage is multiplied (8,192 x 8,192 at 1 token 12.2 us,
+  // two ahead and the next after it 13.0).
+  constexpr bool kTwoAhead = SB == 1;
   int ahead_tile = first, ahead_b = b0;
   auto issue_next = [&](int stage) {
     if (ahead_tile >= row_tiles || b0 >= b1) return false;
@@ -382,7 +385,7 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
     return true;
   };
   issue_next(0);
-  bool more = issue_next(1);  // whether the stage after the one at hand is under way
+  bool more = kTwoAhead && issue_next(1);  // whether the stage after the one at hand is under way
   int stage = 0;
   for (int u = threadIdx.x >> 4; u < blocks * T; u += 32) {
     const int b = u / T, tok = u - b * T, k8 = r, k = b * kBlock + 8 * k8;
@@ -402,6 +405,10 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
     for (int n = 0; n < NA; ++n) total[n] = acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     int slot = 0;
     for (int b = b0; b < b1; b += SB) {
+      if constexpr (!kTwoAhead) {
+        wait_lds();  // the other stage has been read
+        more = issue_next(stage ^ 1);
+      }
       if (more)
         wait_vmcnt<F::kLoads>();
       else
@@ -450,8 +457,10 @@ q4_few_kernel(Q4Out out, const float* __restrict__ x, Q4View w0, Q4View w1, int 
             ++slot;
           }
       }
-      wait_lds();  // the stage has been read
-      more = issue_next(stage);
+      if constexpr (kTwoAhead) {
+        wait_lds();  // the stage has been read
+        more = issue_next(stage);
+      }
       stage ^= 1;
     }
     if constexpr (SPLIT) {
@@ -765,13 +774,11 @@ int check_matrix_q4(const ie_matrix_q4& m, const char* who) {
 constexpr int kFewLds = 160 * 1024;
 
 // Whether the activations are split once into the workspace, by a launch of their own: more than 16
-// tokens, or more than q4_few_kernel holds in LDS beside its stages (57 KB of parts up to 1,024 columns,
-// whose stages are the smaller, 45 KB above).
+// tokens, or more than q4_few_kernel holds in LDS beside its smallest stages (95 KB of parts).
 bool needs_parts(int T, int cols) {
   const int64_t places = T == 1 ? 1 : T <= 4 ? 4 : 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
-  return T > 16 || places * blocks > (blocks <= kSlots ? 112 : 88);
+  return T > 16 || places * blocks > 184;
 }
-
 
 struct Q4Launch {
   Q4Out out;
@@ -806,10 +813,11 @@ struct Q4Launch {
   }
   template <bool GATE, int GROUP, bool S32, int TP>
   bool few(int64_t row_tiles, int64_t cus, int* rc) const {
-    constexpr int kMost = GATE ? 2 : 4;
-    if (row_tiles >= 8 * cus) return few_go<GATE, GROUP, S32, TP, kMost, false>(row_tiles, cus, rc);
-    return cols <= kSlots * kBlock ? few_go<GATE, GROUP, S32, TP, 1, true>(row_tiles, cus, rc)
-                                   : few_go<GATE, GROUP, S32, TP, kMost, true>(row_tiles, cus, rc);
+    constexpr int kMost = GATE ? 2 : 4;  // blocks of a stage, fewer where the tokens' parts need the room
+    if (row_tiles >= 8 * cus && few_go<GATE, GROUP, S32, TP, kMost, false>(row_tiles, cus, rc)) return true;
+    if (cols <= kSlots * kBlock) return few_go<GATE, GROUP, S32, TP, 1, true>(row_tiles, cus, rc);
+    return few_go<GATE, GROUP, S32, TP, kMost, true>(row_tiles, cus, rc) ||
+           few_go<GATE, GROUP, S32, TP, kMost / 2, true>(row_tiles, cus, rc);
   }
   template <bool GATE, int RT, int CT, int GROUP, bool S32>
   int slots() const {

@@ -200,3 +200,22 @@ def test_stream_and_graph(ie, dev):
             torch.cuda.synchronize()
             assert torch.equal(y, wi)
             assert torch.equal(eager(xi), wi)
+
+
+@pytest.mark.parametrize("T,cols", [(1, 23552), (1, 23584), (1, 16384), (2, 5888), (4, 5888), (3, 5920), (16, 1408),
+                                    (9, 1376), (16, 1440), (4, 1024), (12, 1024)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_room_for_the_activations(ie, dev, T, cols, group):
+    """At and past the sizes whose split activations fit beside each stage size: the same bits as the
+    same tokens among many."""
+    rng = np.random.default_rng(cols)
+    m, w = matrix(ie, dev, rng, 75, cols, group, "f16", True)
+    x = activations(rng, 20, cols)
+    got, many = product(ie, dev, m, x[:T]), product(ie, dev, m, x)
+    assert np.array_equal(got.view(np.uint32), many[:T].view(np.uint32))
+    assert (np.abs(got - x[:T].astype(np.float64) @ w.T) <= sum_tolerance(cols, group, w, x[:T])).all()
+    out = [torch.full((t, 75), float("nan"), device=dev) for t in (T, 20)]
+    for o in out:
+        t = o.shape[0]
+        ie.gate_up_silu_q4(o, up(dev, x[:t]), m, m, workspace=ie.matmul_q4_workspace(t, cols, dev))
+    assert torch.equal(out[0], out[1][:T])
