@@ -113,13 +113,13 @@ __device__ __forceinline__ int k8_of(int step, int g) {
   return WIDE ? 4 * g + step : 4 * step + g;
 }
 
-// A block's parts in LDS: 16 bytes per (k8, token), hi then lo, TP token places. Of 16 places they are
-// permuted by k8, so that the 16 lanes that write a token's block hit every bank.
+// A block's parts in LDS: 16 bytes per (k8, token), hi then lo, TP token places. Of 8 and 16 places they
+// are permuted by k8, so that the 16 lanes that write a token's block hit every bank.
 template <int TP>
 struct Places {
   static constexpr int kHalf = 16 * TP * 16, kBytes = 2 * kHalf;
   __device__ __forceinline__ static int at(int k8, int tok) {
-    return (k8 * TP + (TP == 16 ? tok ^ k8 : tok)) * 16;
+    return (k8 * TP + (TP >= 8 ? tok ^ (k8 % TP) : tok)) * 16;
   }
 };
 
@@ -319,7 +319,7 @@ struct FewShape {
 // contiguous bytes of a row a transfer, the next stage under way while one is multiplied. SPLIT: a
 // workgroup takes row tiles in turn, wave i slot i, and the slots are added through LDS. Otherwise (row
 // tiles enough for every wave) a wave takes row tiles of its own, all blocks, folding slots as it passes
-// their ends, and waits for nobody. TP: token places, 1, 4 or 16.
+// their ends, and waits for nobody. TP: token places, 1, 4, 8 or 16.
 // Loads straight to registers touch 16 rows 64 bytes at a time, which bounds them (8,192 x 8,192 at 1
 // token: 22 us so).
 template <bool GATE, int GROUP, bool S32, int TP, int SB, bool SPLIT>
@@ -547,23 +547,36 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   const Q4Rows<RT, GROUP, S32> w[2] = {{w0, scale_type, row0, rows, cols, r},
                                        {GATE ? w1 : w0, scale_type, row0, rows, cols, r}};
   const int b0 = slot_block(wave, blocks), b1 = slot_block(wave + 1, blocks);
-  for (int b = b0; b < b1; ++b) {
-    Q4Block<RT, GROUP, S32> wb[NA];
-#pragma unroll
-    for (int n = 0; n < NA; ++n) wb[n].load(w[n], b, g);
+  struct Ahead {
+    Q4Block<RT, GROUP, S32> w[NA];
     f16x8 hi[CT][4], lo[CT][4];
     f32x4 back[CT];
+  };
+  auto fetch = [&](Ahead& a, int b) {
+#pragma unroll
+    for (int n = 0; n < NA; ++n) a.w[n].load(w[n], b, g);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const size_t at = size_t(min(tok0 / 16 + c, last_tile)) * blocks + b;
       const unsigned char* parts = x.parts + at * kPartBytes;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        hi[c][j] = *reinterpret_cast<const f16x8*>(parts + (lane * 16 + j * 1024));
-        lo[c][j] = *reinterpret_cast<const f16x8*>(parts + (lane * 16 + 4096 + j * 1024));
+        a.hi[c][j] = *reinterpret_cast<const f16x8*>(parts + (lane * 16 + j * 1024));
+        a.lo[c][j] = *reinterpret_cast<const f16x8*>(parts + (lane * 16 + 4096 + j * 1024));
       }
-      back[c] = *reinterpret_cast<const f32x4*>(x.back + at * 16 + 4 * g);
+      a.back[c] = *reinterpret_cast<const f32x4*>(x.back + at * 16 + 4 * g);
     }
+  };
+  constexpr bool kAhead = NA * RT == 1;  // one row tile leaves registers for the next block
+  Ahead next;
+  if (kAhead && b0 < b1) fetch(next, b0);
+  for (int b = b0; b < b1; ++b) {
+    if constexpr (!kAhead) fetch(next, b);
+    const Ahead now = next;
+    if (kAhead && b + 1 < b1) fetch(next, b + 1);
+    const auto& wb = now.w;
+    const auto &hi = now.hi, &lo = now.lo;
+    const auto& back = now.back;
 #pragma unroll
     for (int n = 0; n < NA; ++n)
 #pragma unroll
@@ -603,59 +616,78 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
   }
 }
 
-// A stage of q4_tiles_kernel in LDS: the parts of 8 token tiles, their powers, 8 row tiles' weights with
-// their scales and zero points.
-constexpr int kTileBacks = 8 * kPartBytes, kTileWeights = kTileBacks + 8 * 256, kTileUnit = 1024 + 512;
-constexpr int kTileStage = kTileWeights + 8 * kTileUnit;
+// q4_tiles_kernel's workgroup: WN waves of 32 tokens by 8 / WN of 64 rows (32 of each matrix with GATE), and
+// its stage in LDS: the parts of 2 WN token tiles, their powers, 32 / WN row tiles' weights with their
+// scales and zero points.
+template <bool GATE, int WN>
+struct TilesShape {
+  static constexpr int WM = 8 / WN, kTokens = 32 * WN, kRows = (GATE ? 32 : 64) * WM;
+  static constexpr int kTokTiles = 2 * WN, kRowTiles = 4 * WM;  // of both matrices
+  static constexpr int kBacks = kTokTiles * kPartBytes, kWeights = kBacks + kTokTiles * 256;
+  static constexpr int kUnit = 1024 + 512, kStage = kWeights + kRowTiles * kUnit;
+};
 
-// Prompts: 128 rows (64 of each matrix with GATE) x 128 tokens a workgroup, a wave 64 x 32 of them: 2 x 4
-// waves, two to a SIMD, so that one's VALU work stands beside the other's products (4 waves of 64 x 64,
-// which unpack half as often, one to a SIMD: 4,096 x 4,096 at 2,048 tokens 258 us). A block's parts and
-// weights reach LDS by DMA (73 KB, two stages, the next under way while a block is multiplied). All blocks
-// are walked in turn, the slots' sums folded at their ends.
-template <bool GATE, int GROUP, bool S32>
+// Prompts, and a decode batch against a matrix of many rows: a wave multiplies 64 rows (32 of each matrix)
+// by 32 tokens, two waves to a SIMD, so that one's VALU work stands beside the other's products (4 waves
+// of 64 x 64, which unpack half as often, one to a SIMD: 4,096 x 4,096 at 2,048 tokens 258 us). A block's
+// parts and weights reach LDS by DMA (64 to 78 KB, two stages, the next under way while a block is
+// multiplied: weights straight to registers 248 us, all of a block's transfers issued before its products
+// 172, between them 158). All blocks are walked in turn, the slots' sums folded at their ends. WN: 4 waves
+// of tokens (128), 2 up to 64 tokens, 1 up to 32.
+template <bool GATE, int GROUP, bool S32, int WN>
 __global__ void __launch_bounds__(512)
 q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
                 int row_tiles, int tok_tiles) {
+  using F = TilesShape<GATE, WN>;
   constexpr int NA = GATE ? 2 : 1, RT = 4, CT = 2, RM = RT / NA;  // RM: row tiles per matrix
-  constexpr int kPer = kBlock / GROUP, kSize = S32 ? 4 : 2;
+  constexpr int kPer = kBlock / GROUP, kSize = S32 ? 4 : 2, kMine = F::kRowTiles / 8;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, r = lane & 15, wm = wave >> 2, wn = wave & 3;
+  const int g = lane >> 4, r = lane & 15, wm = wave / WN, wn = wave % WN;
   int row_tile, tok_tile;
   tile_of_block<GATE>(blockIdx.x, row_tiles, tok_tiles, row_tile, tok_tile);
-  const int row0 = (row_tile * 2 + wm) * 16 * RM, tok0 = tok_tile * 128;
+  const int row0 = (row_tile * F::WM + wm) * 16 * RM, tok0 = tok_tile * F::kTokens;
   const int blocks = (cols + kBlock - 1) / kBlock, groups = (cols + GROUP - 1) / GROUP;
   const int last_tile = (T - 1) / 16;
   const bool bf16 = scale_type == IE_KV_BF16;
   const unsigned base = lds_address(dyn);
-  // Wave i brings token tile i of a block (8 transfers of 1 KB, one of powers) and row tile i of the
-  // workgroup's 8 (one each of weights, scales and zero points); waves 4 wm .. 4 wm + 3 use the latter.
-  const size_t part_at = size_t(min(tok_tile * 8 + wave, last_tile)) * blocks;
-  const Q4View& w = GATE && wave % 4 >= RM ? w1 : w0;
-  const int load_row = min((row_tile * 2 + wm) * 16 * RM + wave % RM * 16, rows - 1);
-  const int last_row = rows - 1 - load_row;
-  const uint8_t* data = w.data + size_t(load_row) * (cols / 2);
-  const uint8_t* scale = w.scale + size_t(load_row) * groups * kSize;
-  const uint8_t* zero = w.zero ? w.zero + size_t(load_row) * groups : kEight;
-  const uint32_t zero_step = w.zero ? 1 : 0;
-  const uint32_t data_row = uint32_t(min(lane / 4, last_row)) * (cols / 2);
-  const uint32_t scale_row = uint32_t(min(r, last_row)) * groups;
+  // Of a block, a wave brings 2 WN of the parts' transfers of 1 KB, row tiles wave kMine .. of the
+  // workgroup's (each a transfer of weights, of scales, of zero points), and a token tile's powers. Row
+  // tile 4 wm + i is tile i of the waves wm: of matrix i / RM.
+  const uint8_t *data[kMine], *scale[kMine], *zero[kMine];
+  uint32_t data_row[kMine], scale_row[kMine], zero_step[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int t = wave * kMine + i;
+    const Q4View& w = t % 4 >= RM ? w1 : w0;
+    const int row = min((row_tile * F::WM + t / 4) * 16 * RM + t % RM * 16, rows - 1), last = rows - 1 - row;
+    data[i] = w.data + size_t(row) * (cols / 2);
+    scale[i] = w.scale + size_t(row) * groups * kSize;
+    zero[i] = w.zero ? w.zero + size_t(row) * groups : kEight;
+    zero_step[i] = w.zero ? 1 : 0;
+    data_row[i] = uint32_t(min(lane / 4, last)) * (cols / 2);
+    scale_row[i] = uint32_t(min(r, last)) * groups;
+  }
+  auto token_tile = [&](int t) { return size_t(min(tok_tile * F::kTokTiles + t, last_tile)) * blocks; };
   // In four parts, so that a block's products start before all of the next one's transfers are taken.
   auto issue = [&](int b, int s, int part) {
-    const unsigned to = base + s * kTileStage;
+    const unsigned to = base + s * F::kStage;
 #pragma unroll
-    for (int j = 2 * part; j < 2 * part + 2; ++j)
-      dma16_at(x.parts + (part_at + b) * kPartBytes + j * 1024, lane * 16, to + wave * kPartBytes + j * 1024);
-    if (part > 0) return;
-    dma_word<4>(x.back + (part_at + b) * 16, r * 4, to + kTileBacks + wave * 256);
-    const int word = min(4 * b + ((lane & 3) ^ (lane >> 4)), cols / 32 - 1);
-    const unsigned unit = to + kTileWeights + wave * kTileUnit;
-    dma16_at(data, data_row + word * 16, unit);
-    const uint32_t at = scale_row + min(b * kPer + g * kPer / 4, groups - 1);
-    dma_word<kSize>(scale, at * kSize, unit + 1024);
-    dma_word<1>(zero, at * zero_step, unit + 1280);
+    for (int j = part; j < 2 * WN; j += 4) {
+      const int n = wave * 2 * WN + j;  // of the 16 WN transfers
+      dma16_at(x.parts + (token_tile(n / 8) + b) * kPartBytes + n % 8 * 1024, lane * 16, to + n * 1024);
+    }
+    if (part == 3 && wave < F::kTokTiles)
+      dma_word<4>(x.back + (token_tile(wave) + b) * 16, r * 4, to + F::kBacks + wave * 256);
+    if (part < kMine) {
+      const unsigned unit = to + F::kWeights + (wave * kMine + part) * F::kUnit;
+      const int word = min(4 * b + ((lane & 3) ^ (lane >> 4)), cols / 32 - 1);
+      dma16_at(data[part % kMine], data_row[part % kMine] + word * 16, unit);
+      const uint32_t at = scale_row[part % kMine] + min(b * kPer + g * kPer / 4, groups - 1);
+      dma_word<kSize>(scale[part % kMine], at * kSize, unit + 1024);
+      dma_word<1>(zero[part % kMine], at * zero_step[part % kMine], unit + 1280);
+    }
   };
   f32x4 total[RT][CT], acc[RT][CT];
 #pragma unroll
@@ -673,7 +705,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
     for (; b < b1; ++b) {
       // This wave's transfers have landed, then everyone's, and the other stage has been read.
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      const unsigned char* from = dyn + (b & 1) * kTileStage;
+      const unsigned char* from = dyn + (b & 1) * F::kStage;
       const unsigned char* parts = from + 2 * wn * kPartBytes + lane * 16;
       f16x8 hi[2][CT], lo[2][CT];
       auto read = [&](int j) {
@@ -686,7 +718,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
       read(0);
       using Tile = Q4Tile<GROUP, S32>;
       auto tile = [&](int i) {
-        const unsigned char* unit = from + kTileWeights + (4 * wm + i) * kTileUnit;
+        const unsigned char* unit = from + F::kWeights + (4 * wm + i) * F::kUnit;
         const u32x4 q = *reinterpret_cast<const u32x4*>(unit + (r * 4 + (g ^ (r >> 2))) * 16);
         uint32_t sc[kPer], ze[kPer];
 #pragma unroll
@@ -720,7 +752,7 @@ q4_tiles_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
         if ((j + 1) % (4 / kPer) == 0) {
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
-            const f32x4 back = *reinterpret_cast<const f32x4*>(from + kTileBacks + (2 * wn + c) * 256 + 16 * g);
+            const f32x4 back = *reinterpret_cast<const f32x4*>(from + F::kBacks + (2 * wn + c) * 256 + 16 * g);
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -776,7 +808,7 @@ constexpr int kFewLds = 160 * 1024;
 // Whether the activations are split once into the workspace, by a launch of their own: more than 16
 // tokens, or more than q4_few_kernel holds in LDS beside its smallest stages (95 KB of parts).
 bool needs_parts(int T, int cols) {
-  const int64_t places = T == 1 ? 1 : T <= 4 ? 4 : 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
+  const int64_t places = T == 1 ? 1 : T <= 4 ? 4 : T <= 8 ? 8 : 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
   return T > 16 || places * blocks > 184;
 }
 
@@ -831,17 +863,25 @@ struct Q4Launch {
                        int(row_groups), int(tok_groups));
     return IE_HIP_OK;
   }
-  template <bool GATE, int GROUP, bool S32>
-  int tiles() const {
-    constexpr int kLds = 2 * kTileStage, kRows = GATE ? 64 : 128;
-    const auto kernel = q4_tiles_kernel<GATE, GROUP, S32>;
-    static const int rc = more_lds(kernel, kLds);
-    if (rc) return rc;
-    const int64_t row_tiles = (int64_t(rows) + kRows - 1) / kRows, tok_tiles = (int64_t(T) + 127) / 128;
-    if (row_tiles * tok_tiles * 512 > int64_t(UINT32_MAX)) return too_many();
+  // False where the tiles leave half of the compute units without one.
+  template <bool GATE, int GROUP, bool S32, int WN>
+  bool tiles(int64_t cus, int* rc) const {
+    using F = TilesShape<GATE, WN>;
+    constexpr int kLds = 2 * F::kStage;
+    static_assert(kLds <= 160 * 1024, "a compute unit's LDS");
+    const int64_t row_tiles = (int64_t(rows) + F::kRows - 1) / F::kRows;
+    const int64_t tok_tiles = (int64_t(T) + F::kTokens - 1) / F::kTokens;
+    if (2 * row_tiles * tok_tiles < cus) return false;
+    const auto kernel = q4_tiles_kernel<GATE, GROUP, S32, WN>;
+    static const int more = more_lds(kernel, kLds);
+    if ((*rc = more)) return true;
+    if (row_tiles * tok_tiles * 512 > int64_t(UINT32_MAX)) {
+      *rc = too_many();
+      return true;
+    }
     hipLaunchKernelGGL(kernel, dim3(unsigned(row_tiles * tok_tiles)), dim3(512), kLds, stream, out, parts,
                        w0, w1, scale_type, T, rows, cols, int(row_tiles), int(tok_tiles));
-    return IE_HIP_OK;
+    return true;
   }
   template <bool GATE, int GROUP, bool S32>
   int run() const {
@@ -850,8 +890,9 @@ struct Q4Launch {
     int rc = IE_HIP_OK;
     if (!needs_parts(T, cols)) {
       if (T == 1 ? few<GATE, GROUP, S32, 1>(row_tiles, cus, &rc)
-                 : T <= 4 ? few<GATE, GROUP, S32, 4>(row_tiles, cus, &rc)
-                          : few<GATE, GROUP, S32, 16>(row_tiles, cus, &rc))
+          : T <= 4 ? few<GATE, GROUP, S32, 4>(row_tiles, cus, &rc)
+          : T <= 8 ? few<GATE, GROUP, S32, 8>(row_tiles, cus, &rc)
+                   : few<GATE, GROUP, S32, 16>(row_tiles, cus, &rc))
         return rc;
       return fail(IE_HIP_EINVAL, std::string(who) + ": activations past a workgroup's memory");
     }
@@ -859,8 +900,9 @@ struct Q4Launch {
     if (tok_tiles * blocks * 256 > int64_t(UINT32_MAX)) return too_many();
     hipLaunchKernelGGL(q4_split_kernel<GROUP == kBlock>, dim3(unsigned(tok_tiles * blocks)), dim3(256), 0,
                        stream, parts, x, T, cols, int(blocks));
-    const int64_t big = ((int64_t(rows) + (GATE ? 63 : 127)) / (GATE ? 64 : 128)) * ((int64_t(T) + 127) / 128);
-    if (2 * big >= cus) return tiles<GATE, GROUP, S32>();
+    if (T <= 32 ? tiles<GATE, GROUP, S32, 1>(cus, &rc)
+                : T <= 64 ? tiles<GATE, GROUP, S32, 2>(cus, &rc) : tiles<GATE, GROUP, S32, 4>(cus, &rc))
+      return rc;
     constexpr int kMost = GATE ? 2 : 4;  // row tiles of a workgroup: as many as leave every unit one
     if ((row_tiles + kMost - 1) / kMost * tok_tiles >= cus) return slots<GATE, kMost, 1, GROUP, S32>();
     if (!GATE && (row_tiles + 1) / 2 * tok_tiles >= cus) return slots<GATE, 2, 1, GROUP, S32>();
