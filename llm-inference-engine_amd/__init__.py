@@ -60,6 +60,7 @@ class MatrixQ4(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("zero", ctypes.c_void_p),
                 ("scale_dtype", ctypes.c_int32), ("group", ctypes.c_int32),
                 ("rows", ctypes.c_int32), ("cols", ctypes.c_int32)]
+    tensors, device = (), -1  # set by matrix_q4()
 
 
 class LogitRules(ctypes.Structure):
@@ -70,6 +71,7 @@ class LogitRules(ctypes.Structure):
         "frequency", "bias_token", "bias_value", "bias_start", "bias_len", "mask", "mask_row")]
         + [("history_size", ctypes.c_int64), ("bias_size", ctypes.c_int64),
            ("mask_rows", ctypes.c_int32)])
+    tensors, rows, words = (), None, None  # set by logit_rules()
 
 
 _vp, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float

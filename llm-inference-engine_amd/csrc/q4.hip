@@ -18,6 +18,7 @@
 // Lane (g, r) of a tile of 16 rows x 16 tokens loads 16 bytes = 32 columns of row r at a time, and
 // holds the results of tokens 4g .. 4g+3 and row r, so that a lane meets one scale per group.
 #include <algorithm>
+#include <atomic>
 
 #include "common.hpp"
 #include "matmul_tiled.hpp"
@@ -522,7 +523,7 @@ q4_split_kernel(Parts out, const float* __restrict__ x, int T, int cols, int blo
 // RT row tiles (of each matrix) by CT tiles of 16 tokens, the tokens' parts straight from the workspace and
 // held while the row tiles go past them, then the slots are added through LDS. What a launch reads over and
 // over is the parts (once per group of row tiles), so row tiles come before token tiles: q/k/v of 300
-// tokens 1 x 4 tiles 10.1 us, RTxCT us; a workgroup's registers leave room for a second one.
+// tokens 1 x 4 tiles 10.1 us, 4 x 1 8.5; a workgroup's registers leave room for a second one.
 template <bool GATE, int RT, int CT, int GROUP, bool S32>
 __global__ void __launch_bounds__(64 * kSlots, 4)
 q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
@@ -822,11 +823,19 @@ struct Q4Launch {
   const char* who;
 
   int too_many() const { return fail(IE_HIP_EINVAL, std::string(who) + ": too many rows or tokens"); }
+  // Raises a kernel's dynamic-LDS cap, once on each device: `done` is the kernel's own, a bit a device.
   template <class Kernel>
-  int more_lds(Kernel kernel, int bytes) const {
-    return check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                         hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
-                     "hipFuncSetAttribute(q4)");
+  int more_lds(Kernel kernel, int bytes, std::atomic<uint64_t>& done) const {
+    int device = 0;
+    if (int rc = check_hip(hipGetDevice(&device), "hipGetDevice")) return rc;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_relaxed) & bit)) return IE_HIP_OK;
+    if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                           "hipFuncSetAttribute(q4)"))
+      return rc;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return IE_HIP_OK;
   }
   // False where the tokens' parts do not fit.
   template <bool GATE, int GROUP, bool S32, int TP, int SB, bool SPLIT>
@@ -835,8 +844,8 @@ struct Q4Launch {
     const int64_t lds = F::bytes((int64_t(cols) + kBlock - 1) / kBlock);
     if (lds > kFewLds) return false;
     const auto kernel = q4_few_kernel<GATE, GROUP, S32, TP, SB, SPLIT>;
-    static const int more = more_lds(kernel, kFewLds);
-    if ((*rc = more)) return true;
+    static std::atomic<uint64_t> done{0};
+    if ((*rc = more_lds(kernel, kFewLds, done))) return true;
     const int64_t each = std::min<int64_t>(2, kFewLds / lds);  // workgroups of a compute unit
     const int64_t grid = std::min(SPLIT ? row_tiles : (row_tiles + kSlots - 1) / kSlots, each * cus);
     hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(64 * kSlots), unsigned(lds), stream, out, x, w0,
@@ -873,8 +882,8 @@ struct Q4Launch {
     const int64_t tok_tiles = (int64_t(T) + F::kTokens - 1) / F::kTokens;
     if (2 * row_tiles * tok_tiles < cus) return false;
     const auto kernel = q4_tiles_kernel<GATE, GROUP, S32, WN>;
-    static const int more = more_lds(kernel, kLds);
-    if ((*rc = more)) return true;
+    static std::atomic<uint64_t> done{0};
+    if ((*rc = more_lds(kernel, kLds, done))) return true;
     if (row_tiles * tok_tiles * 512 > int64_t(UINT32_MAX)) {
       *rc = too_many();
       return true;

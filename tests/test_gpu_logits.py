@@ -362,3 +362,74 @@ def test_sample_wide_borders(ie, dev):
     m, p, k = 10.0 ** -rng.uniform(1, 5, R), 0.3 + 0.69 * rng.random(R), rng.integers(2000, 140000, R)
     for kk, pp, mm in ((None, None, m), (None, p, m), (k, None, None), (k, p, None), (k, p, m), (None, p, None)):
         assert draw(ie, dev, l, t, u, kk, pp, mm).tolist() == expect(l, t, u, kk, pp, mm)
+
+
+def test_sample_largest_vocabulary(ie, dev):
+    """4,194,304 tokens, a row of few values and one of many; one more token is refused."""
+    rng = np.random.default_rng(4)
+    n = 1 << 22
+    l = np.zeros((2, n), np.float32)
+    l[0, rng.integers(0, n, n // 3)] = 1.0
+    l[1] = rng.standard_normal(n, dtype=np.float32)
+    t, u = np.ones(2), np.array([0.83, 0.41])
+    for k, p in ((None, None), ([1500000, 0], [1.0, 0.4]), ([3000000, 7], [0.6, 0.9])):
+        assert draw(ie, dev, l, t, u, k, p).tolist() == expect(l, t, u, k, p)
+    assert ie.lib().ie_hip_sample_rows_workspace_bytes(1, n + 1) == 0
+    big = torch.zeros((1, n + 1), device=dev)
+    one = torch.zeros(1, device=dev)
+    with pytest.raises(ie.IeHipError, match="4,194,304"):
+        ie.sample_rows(torch.zeros(1, dtype=torch.int32, device=dev), big, one, one,
+                       workspace=ie.sample_rows_workspace(1, n, dev))
+
+
+def test_two_streams_at_once(ie, dev):
+    """Calls on two streams with workspaces of their own, and a workspace made for more rows."""
+    rng = np.random.default_rng(21)
+    R, n = 16, 70001
+    ls = [rows_of_logits(rng, R, n) for _ in range(2)]
+    t, u, p = 0.5 + rng.random(R), rng.random(R), 0.5 + 0.5 * rng.random(R)
+    f32 = lambda a: up(dev, np.asarray(a, np.float32))
+    dl, dt, du, dp = [up(dev, l) for l in ls], f32(t), f32(u), f32(p)
+    ws = [ie.sample_rows_workspace(64, 100000, dev) for _ in range(2)]
+    outs = [torch.full((R,), -1, dtype=torch.int32, device=dev) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(2):
+            ie.sample_rows(outs[i], dl[i], dt, du, top_p=dp, workspace=ws[i], stream=streams[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert outs[i].tolist() == expect(ls[i], t, u, None, p)
+
+
+def test_calls_refuse_what_does_not_fit(ie, dev):
+    z = lambda *s, **k: torch.zeros(*s, device=dev, **k)
+    i32 = torch.int32
+    l, one = z(2, 100), z(2)
+    out = z(2, dtype=i32)
+    for bad in (dict(workspace=None), dict(workspace=z(16, dtype=torch.uint8)), dict(top_k=z(3, dtype=i32)),
+                dict(top_p=z(2, dtype=torch.float64)), dict(min_p=z(2, 1))):
+        with pytest.raises(ie.IeHipError):
+            ie.sample_rows(out, l, one, one, **{"workspace": ie.sample_rows_workspace(2, 100, dev), **bad})
+    with pytest.raises(ie.IeHipError, match="contiguous"):
+        ie.sample_rows(out, z(100, 2).t(), one, one, workspace=ie.sample_rows_workspace(2, 100, dev))
+    with pytest.raises(ie.IeHipError, match="words"):
+        ie.adjust_logits(l, l, ie.logit_rules(mask=z(2, 3, dtype=i32)))
+    rules = ie.logit_rules(history=(z(4, dtype=i32), z(3, dtype=i32), z(3, dtype=i32)))
+    with pytest.raises(ie.IeHipError, match="rows"):
+        ie.adjust_logits(l, l, rules)
+    with pytest.raises(ie.IeHipError, match="shape"):
+        ie.adjust_logits(z(2, 99), l, ie.logit_rules())
+    w = ie.matrix_q4(z(16, 16, dtype=torch.uint8), z(16, 1), 32)
+    x, y = z(40, 32), z(40, 16)
+    with pytest.raises(ie.IeHipError, match="workspace"):
+        ie.matmul_q4(y, x, w)
+    for args in ((z(40, 15), x, w), (y, z(40, 64), w), (z(39, 16), x, w), (y, x, w, z(15)),
+                 (y, x.cpu(), w), (y.cpu(), x, w), (y.half(), x, w)):
+        with pytest.raises(ie.IeHipError):
+            ie.matmul_q4(*args, workspace=ie.matmul_q4_workspace(40, 32, dev))
+    ie.matmul_q4(z(0, 16), z(0, 32), w)
+    ie.sample_rows(z(0, dtype=i32), z(0, 100), z(0), z(0))
+    vec = z(16) + 9
+    ie.matmul_q4(vec, z(32), w)  # one token as a vector
+    assert not vec.any()

@@ -97,6 +97,8 @@ def test_python_refuses_other_tensors(ie):
     assert (w.rows, w.cols, w.group, w.scale_dtype) == (4, 64, 32, ie.KV_F32)
     with pytest.raises(ie.IeHipError, match="current GPU"):
         ie.matmul_q4(z(1, 4), z(1, 64), w, stream=STREAM)
+    with pytest.raises(ie.IeHipError, match="current GPU"):  # a structure of the caller's own
+        ie.matmul_q4(z(1, 4), z(1, 64), q4(ie, rows=4), stream=STREAM)
     with pytest.raises(ie.IeHipError, match="float32"):
         ie.matmul_q4(z(1, 4), z(1, 64, dtype=torch.float16), w, stream=STREAM)
     with pytest.raises(ie.IeHipError, match="contiguous"):
