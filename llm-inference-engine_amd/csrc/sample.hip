@@ -30,7 +30,7 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the launches over rows
 constexpr int kChunkThreads = 512, kEach = 8;           // of those over chunks, and logits of a thread
 constexpr int kChunk = kChunkThreads * kEach;
-constexpr int kPlaces = 512;               // bins of the rows' histograms, a thread each of `border`
+constexpr int kPlaces = 512;               // bins of the rows' histograms
 constexpr int kList = 6144;                // border tokens of a row
 constexpr int kDigits = 2048;
 constexpr int kMaxTokens = 1 << 22, kMaxChunks = kMaxTokens / kChunk;
@@ -346,12 +346,13 @@ __device__ __forceinline__ T running(u64 (&sh)[WAVES], T x) {
   return x;
 }
 
-__global__ void __launch_bounds__(kPlaces)
+__global__ void __launch_bounds__(kThreads)
 sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, int chunks, double one) {
+  static_assert(kThreads == 2 * kPlaces, "a bin is two threads'");
   __shared__ uint32_t count[kPlaces];
   __shared__ u64 mass[kPlaces];
   __shared__ double powers[64];
-  __shared__ u64 sh[kPlaces / 64];
+  __shared__ u64 sh[kWaves];
   __shared__ int found[3];
   __shared__ double factor[kMaxChunks];
   __shared__ int shift[kMaxChunks];
@@ -362,13 +363,13 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   if (tid < 3) found[tid] = kPlaces - 1;
   fill_powers(powers);
   u64 best = 0;
-  for (int c = tid; c < chunks; c += kPlaces) best = tops[c] > best ? tops[c] : best;
+  for (int c = tid; c < chunks; c += kThreads) best = tops[c] > best ? tops[c] : best;
   best = wave_best(best);
   if (lane == 0) sh[wave] = best;
   __syncthreads();
   best = 0;
 #pragma unroll
-  for (int i = 0; i < kPlaces / 64; ++i) best = sh[i] > best ? sh[i] : best;
+  for (int i = 0; i < kWaves; ++i) best = sh[i] > best ? sh[i] : best;
   const float largest = candidate_logit(best);
   const bool infinite = largest == INFINITY;
   const float top = infinite ? 0.0f : largest;
@@ -383,36 +384,52 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
     return;
   }
   const double tp = place(top, r.scale);
-  for (int c = tid; c < chunks; c += kPlaces) {
+  for (int c = tid; c < chunks; c += kThreads) {
     const float t = in_row(candidate_logit(tops[c]), infinite);
     factor[c] = weight_of(t, top, r.rate, powers);
     sums[c] = r.p < 1.0f ? rescale(w.mass[size_t(row) * chunks + c], factor[c]) : 0;
     shift[c] = t > -INFINITY ? bin_below(tp, t, r.scale) : kPlaces;
   }
   __syncthreads();
-  // This thread's bin over the chunks: each has it further down by how far its own top is below the
-  // row's. The last bin is what the others leave, so nothing is added up from several bins.
+  // A bin over the chunks, every other one by each of two threads: a chunk has it further down by how far
+  // its own top is below the row's. The last bin is what the others leave, so nothing is added up from
+  // several bins.
   const bool by_count = r.k < n, by_mass = r.p < 1.0f;
+  const int place_of = tid % kPlaces, half = tid / kPlaces;
   u64 own_m = 0, all = 0;
   uint32_t own_n = 0;
-  constexpr int kBatch = 20;  // loads under way at once
-  auto gather = [&](const auto* bins, const auto& add) {
-    for (int c0 = 0; c0 < chunks; c0 += kBatch) {
-      std::decay_t<decltype(*bins)> got[kBatch];
+  auto gather = [&](auto with_mass, auto with_count) {
+    constexpr bool MASS = decltype(with_mass)::value, COUNT = decltype(with_count)::value;
+    constexpr int kBatch = 10;  // loads of either kind under way at once
+    for (int c0 = half; c0 < chunks; c0 += 2 * kBatch) {
+      u64 m[kBatch];
+      uint32_t k[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int c = min(c0 + j, chunks - 1);
-        got[j] = bins[(size_t(row) * chunks + c) * kPlaces + max(tid - shift[c], 0)];
+        const int c = min(c0 + 2 * j, chunks - 1);
+        const size_t at = (size_t(row) * chunks + c) * kPlaces + max(place_of - shift[c], 0);
+        if constexpr (MASS) m[j] = w.bin_mass[at];
+        if constexpr (COUNT) k[j] = w.bin_count[at];
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int c = min(c0 + j, chunks - 1);
-        if (c0 + j < chunks && tid >= shift[c]) add(got[j], c);
+        const int c = min(c0 + 2 * j, chunks - 1);
+        const bool in = c0 + 2 * j < chunks && place_of >= shift[c];
+        if constexpr (MASS) own_m += in ? rescale(m[j], factor[c]) : 0;
+        if constexpr (COUNT) own_n += in ? k[j] : 0;
       }
     }
   };
-  if (by_mass) gather(w.bin_mass, [&](u64 m, int c) { own_m += rescale(m, factor[c]); });
-  if (by_count) gather(w.bin_count, [&](uint32_t c, int) { own_n += c; });
+  if (by_mass && by_count)
+    gather(std::true_type{}, std::true_type{});
+  else if (by_mass)
+    gather(std::true_type{}, std::false_type{});
+  else if (by_count)
+    gather(std::false_type{}, std::true_type{});
+  if (half) count[place_of] = own_n, mass[place_of] = own_m;
+  __syncthreads();
+  own_n = half ? 0 : own_n + count[place_of];
+  own_m = half ? 0 : own_m + mass[place_of];
   if (by_mass) {
     for (int c = lane; c < chunks; c += 64) all += sums[c];
     all = wave_sum(all);
@@ -426,14 +443,14 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
     cm += own_m;
     cn = uint32_t(n);
   }
-  count[tid] = cn;  // running sums from here on
-  mass[tid] = cm;
+  __syncthreads();
+  if (!half) count[tid] = cn, mass[tid] = cm;  // running sums from here on
   const u64 bm = cm - own_m;
   const uint32_t bn = cn - own_n;
   // top-k's bin: the one in which the running count reaches k
-  if (bn < uint32_t(r.k) && cn >= uint32_t(r.k)) found[0] = tid;
+  if (!half && bn < uint32_t(r.k) && cn >= uint32_t(r.k)) found[0] = tid;
   __syncthreads();
-  // The last bin's weights are 0 (e^-31.97 of the largest is less than half of 2^-45), so nobody asks
+  // The last bin's weights are 0 (e^-32.38 of the largest is less than half of 2^-45), so nobody asks
   // which of its tokens are kept, and a border there is none.
   int lo = 0x7fffffff, hi = -1, left = 0x7fffffff;
   if (r.least > 0.0) {
@@ -458,8 +475,8 @@ sample_border_kernel(int32_t* __restrict__ out, Settings s, Workspace w, int n, 
   const u64 above = outer ? mass[hi] : total;
   if (r.p < 1.0f) {
     const double glo = double(r.p) * double(below), ghi = double(r.p) * double(above);
-    if ((tid == 0 || double(bm) < glo) && double(cm) >= glo) found[1] = tid;
-    if ((tid == 0 || double(bm) < ghi) && double(cm) >= ghi) found[2] = tid;
+    if (!half && (tid == 0 || double(bm) < glo) && double(cm) >= glo) found[1] = tid;
+    if (!half && (tid == 0 || double(bm) < ghi) && double(cm) >= ghi) found[2] = tid;
   }
   __syncthreads();
   if (tid != 0) return;
@@ -886,7 +903,7 @@ extern "C" int ie_hip_sample_rows(int32_t* out, const float* logits, const float
   const auto each = vec ? sample_chunks_kernel<true> : sample_chunks_kernel<false>;
   const auto collect = vec ? sample_collect_kernel<true> : sample_collect_kernel<false>;
   hipLaunchKernelGGL(each, every, wide, 0, stream, logits, s, w, n, chunks, one);
-  hipLaunchKernelGGL(sample_border_kernel, rows, dim3(kPlaces), 0, stream, out, s, w, n, chunks, one);
+  hipLaunchKernelGGL(sample_border_kernel, rows, block, 0, stream, out, s, w, n, chunks, one);
   if (top_k || top_p || min_p)
     hipLaunchKernelGGL(collect, every, wide, 0, stream, logits, s, w, n, chunks, one);
   hipLaunchKernelGGL(sample_draw_kernel, rows, block, 0, stream, out, logits, s, w, n, chunks, one);
