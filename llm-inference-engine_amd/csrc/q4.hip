@@ -872,7 +872,10 @@ struct Q4Launch {
                        int(row_groups), int(tok_groups));
     return IE_HIP_OK;
   }
-  // False where the tiles leave half of the compute units without one.
+  // False where the tiles, one a compute unit, are so few that the slots take less time: theirs grows with
+  // the launch, the tiles' hardly until every unit has one. Tiles and slots, us: 117 tiles of 896 columns
+  // 27.8 and 26.3, 135 28.3 and 30.0; 96 tiles of 2,048 columns 42.4 and 42.6, 112 42.3 and 48.5; 112 of
+  // 4,096 72.2 and 98.0.
   template <bool GATE, int GROUP, bool S32, int WN>
   bool tiles(int64_t cus, int* rc) const {
     using F = TilesShape<GATE, WN>;
@@ -880,7 +883,7 @@ struct Q4Launch {
     static_assert(kLds <= 160 * 1024, "a compute unit's LDS");
     const int64_t row_tiles = (int64_t(rows) + F::kRows - 1) / F::kRows;
     const int64_t tok_tiles = (int64_t(T) + F::kTokens - 1) / F::kTokens;
-    if (2 * row_tiles * tok_tiles < cus) return false;
+    if ((cols < 2048 ? 2.0 : 2.5) * double(row_tiles * tok_tiles) < double(cus)) return false;
     const auto kernel = q4_tiles_kernel<GATE, GROUP, S32, WN>;
     static std::atomic<uint64_t> done{0};
     if ((*rc = more_lds(kernel, kLds, done))) return true;

@@ -119,6 +119,19 @@ def test_a_token_does_not_depend_on_its_batch(ie, dev):
         assert np.array_equal(alone, want[399:])
 
 
+@pytest.mark.parametrize("cols", [1952, 2080])
+@pytest.mark.parametrize("group", [32, 128])
+def test_many_tokens_on_both_sides_of_a_rule(ie, dev, cols, group):
+    """108 tiles of 128 x 128, which one count of columns takes as tiles and the other by slots: bit for
+    bit what the tokens are eight at a time."""
+    rng = np.random.default_rng(cols + group)
+    m, _ = matrix(ie, dev, rng, 1501, cols, group, zero=True)
+    x = activations(rng, 1030, cols)
+    got = product(ie, dev, m, x).view(np.uint32)
+    for t in (0, 511, 1022):
+        assert np.array_equal(got[t:t + 8], product(ie, dev, m, x[t:t + 8]).view(np.uint32)), t
+
+
 def test_every_weight_and_zero_point(ie, dev):
     """All 16 values against zero points to 255, one column at a time: exact."""
     q = np.tile(np.arange(16, dtype=np.uint8), 2)[None].repeat(256, 0)
