@@ -15,8 +15,8 @@
 //   collect  per chunk the weight of the bins above all borders; the tokens of the border bins go to
 //            the row's list
 //   draw     the borders, found digit by digit of the ordered bit pattern in that list (of at most
-//            kList tokens; the whole row where the bins hold more, as with a row of equal logits),
-//            then the chunk and the token where the running sum passes the target
+//            kHeld tokens, in LDS up to kList; the whole row where the bins hold more, as with a row of
+//            equal logits), then the chunk and the token where the running sum passes the target
 // (64 rows x 151,936, settings mixed: one workgroup a row through all of it took 1,440 us.)
 #include <algorithm>
 #include <cmath>
@@ -31,7 +31,9 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the launches over 
 constexpr int kChunkThreads = 512, kEach = 8;           // of those over chunks, and logits of a thread
 constexpr int kChunk = kChunkThreads * kEach;
 constexpr int kPlaces = 512;               // bins of the rows' histograms
-constexpr int kList = 6144;                // border tokens of a row
+// Border tokens of a row: in LDS, in the workspace (1 x 151,936 of logits in steps of a half, at T = 5
+// with top-p: 12,000 in one bin, 60 us from the workspace, 646 by walks of the row).
+constexpr int kList = 6144, kHeld = 32768;
 constexpr int kDigits = 2048;
 constexpr int kMaxTokens = 1 << 22, kMaxChunks = kMaxTokens / kChunk;
 typedef unsigned long long u64;
@@ -65,7 +67,7 @@ struct Entry {
 
 struct Workspace {
   RowState* rows;    // [R]
-  Entry* list;       // [R, kList]
+  Entry* list;       // [R, kHeld]
   u64* mass;         // [R, chunks] relative to the chunk's own top; after `collect` its sure weight
   u64* top;          // [R, chunks] the largest logit and its place (candidate)
   u64* bin_mass;     // [R, chunks, kPlaces]
@@ -82,7 +84,7 @@ size_t lay_out(Workspace* w, void* base, int R, int n) {
   };
   Workspace v;
   v.rows = reinterpret_cast<RowState*>(take(R * sizeof(RowState)));
-  v.list = reinterpret_cast<Entry*>(take(R * size_t(kList) * sizeof(Entry)));
+  v.list = reinterpret_cast<Entry*>(take(R * size_t(kHeld) * sizeof(Entry)));
   v.mass = reinterpret_cast<u64*>(take(rc * 8));
   v.top = reinterpret_cast<u64*>(take(rc * 8));
   v.bin_mass = reinterpret_cast<u64*>(take(rc * kPlaces * 8));
@@ -567,11 +569,11 @@ sample_collect_kernel(const float* __restrict__ logits, Settings s, Workspace w,
   }
   __syncthreads();
   at += next;
-  Entry* list = w.list + size_t(row) * kList;
+  Entry* list = w.list + size_t(row) * kHeld;
 #pragma unroll
   for (int j = 0; j < kEach; ++j)
     if (listed >> j & 1) {
-      if (at < kList) list[at] = Entry{v[j], base + chunk_index(j)};
+      if (at < kHeld) list[at] = Entry{v[j], base + chunk_index(j)};
       ++at;
     }
 }
@@ -641,7 +643,7 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   if (st.mode == kDone) return;
   const float* l = logits + size_t(row) * n;
   const Row r(s, row, n, one);
-  const bool filtered = st.mode != kAll, all = filtered && st.listed > kList;
+  const bool filtered = st.mode != kAll, all = filtered && st.listed > kHeld;
   const bool infinite = st.top == INFINITY;
   if (infinite) st.top = 0.0f;
   const double tp = place(st.top, r.scale);
@@ -652,8 +654,10 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
     st.top_left = r.k < n ? r.k : 0x7fffffff;
   }
   const int items = !filtered ? 0 : all ? n : st.listed;
-  if (filtered && !all)
-    for (int i = tid; i < items; i += kThreads) list[i] = w.list[size_t(row) * kList + i];
+  const bool in_lds = items <= kList;
+  const Entry* held = w.list + size_t(row) * kHeld;
+  if (!all && in_lds)
+    for (int i = tid; i < items; i += kThreads) list[i] = held[i];
   for (int i = tid; i < chunks; i += kThreads) {
     const size_t rc = size_t(row) * chunks + i;
     chunk_mass[i] = filtered && !all ? w.mass[rc] : 0;
@@ -663,9 +667,9 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
   int digits = 3;
   uint32_t common_prefix = 0;
   if (filtered && !all && items > 0) {
-    const uint32_t o = order_key(list[0].l);
+    const uint32_t o = order_key(held[0].l);
     uint32_t differ = 0;
-    for (int i = tid; i < items; i += kThreads) differ |= order_key(list[i].l) ^ o;
+    for (int i = tid; i < items; i += kThreads) differ |= order_key(in_lds ? list[i].l : held[i].l) ^ o;
     if (tid == 0) chosen = 0;
     __syncthreads();
     if (differ) atomicOr(&chosen, int(differ));
@@ -674,7 +678,9 @@ sample_draw_kernel(int32_t* __restrict__ out, const float* __restrict__ logits, 
     digits = any >> 21 ? 3 : any >> 10 ? 2 : 1;
     common_prefix = digits == 3 ? 0 : digits == 2 ? o >> 21 : o >> 10;
   }
-  auto entry = [&](int i) { return all ? Entry{in_row(read_logit(l[i]), infinite), i} : list[i]; };
+  auto entry = [&](int i) {
+    return all ? Entry{in_row(read_logit(l[i]), infinite), i} : in_lds ? list[i] : held[i];
+  };
   auto bin_of = [&](float v) { return v > -INFINITY ? bin_below(tp, v, r.scale) : kPlaces - 1; };
   auto weight = [&](float v) { return weight_of(v, st.top, r.rate, powers); };
 

@@ -172,6 +172,25 @@ def test_sample_ties(ie, dev, n):
         assert draw(ie, dev, l, t, u, k=kk, p=[0.5] * 8).tolist() == expect(l, t, u, k=kk, p=[0.5] * 8)
 
 
+@pytest.mark.parametrize("many", [6143, 6144, 6145, 32767, 32768, 32769])
+def test_sample_border_of_many_tokens(ie, dev, many):
+    """So many tokens of two near logits at random places, all in one bin, the others far below: what
+    a border's list holds in LDS, in the workspace, and not at all."""
+    n = 40007
+    rng = np.random.default_rng(many)
+    l = np.full((6, n), -50, np.float32)
+    for r in range(6):
+        at = rng.permutation(n)[:many]
+        l[r, at] = np.where(rng.random(many) < 0.5, 1.0, np.float32(1.0 + 2.0 ** -20))
+    t, u = np.ones(6), rng.random(6)
+    k = np.array([1, 2, many // 3, many - 1, many, many + 1], np.int32)
+    p = np.array([1e-6, 0.2, 0.5, 0.75, 0.999, 0.4])
+    m = np.full(6, 0.1)
+    assert draw(ie, dev, l, t, u, k=k).tolist() == expect(l, t, u, k=k)
+    assert draw(ie, dev, l, t, u, p=p).tolist() == expect(l, t, u, p=p)
+    assert draw(ie, dev, l, t, u, k, p, m).tolist() == expect(l, t, u, k, p, m)
+
+
 @pytest.mark.parametrize("n", [7, 5000, 151936])
 def test_sample_odd_values(ie, dev, n):
     """Settings and random numbers outside their ranges; rows of nothing, of one token, of
