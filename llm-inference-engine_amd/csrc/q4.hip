@@ -519,14 +519,42 @@ q4_split_kernel(Parts out, const float* __restrict__ x, int T, int cols, int blo
   if (k8 == 0) out.back[(tile * blocks + b) * 16 + t] = back;
 }
 
+// What the split kernel leaves of a tile of tokens and a block, to the same bits, made by the wave itself:
+// a lane has 32 columns of token `tok`.
+template <bool WIDE>
+__device__ __forceinline__ void split_tile(f16x8 (&hi)[4], f16x8 (&lo)[4], f32x4& back, const float* x,
+                                           int tok, int T, int cols, int b, int g) {
+  float v[4][8];
+  uint32_t largest = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k = b * kBlock + 8 * k8_of<WIDE>(j, g);
+    const bool in = tok < T && k < cols;
+    load8(v[j], x + (in ? size_t(tok) * cols + k : 0), in);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = max(largest, finite_bits(v[j][i]));
+#pragma unroll
+  for (int off = 32; off > 8; off >>= 1) largest = max(largest, uint32_t(__shfl_xor(int(largest), off, 64)));
+  float factor, mine;
+  block_scale(largest, factor, mine);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) split8(v[j], factor, hi[j], lo[j]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) back[e] = __shfl(mine, 4 * g + e, 64);
+}
+
 // More tokens than q4_few_kernel's, fewer than fill the chip with q4_tiles_kernel's: wave i takes slot i of
-// RT row tiles (of each matrix) by CT tiles of 16 tokens, the tokens' parts straight from the workspace and
-// held while the row tiles go past them, then the slots are added through LDS. What a launch reads over and
-// over is the parts (once per group of row tiles), so row tiles come before token tiles: q/k/v of 300
-// tokens 1 x 4 tiles 10.1 us, 4 x 1 8.5; a workgroup's registers leave room for a second one.
-template <bool GATE, int RT, int CT, int GROUP, bool S32>
+// RT row tiles (of each matrix) by CT tiles of 16 tokens, the tokens' parts straight from the workspace
+// (DIRECT: split by the wave) and held while the row tiles go past them, then the slots are added through
+// LDS. What a launch reads over and over is the parts (once per group of row tiles), so row tiles come
+// before token tiles: q/k/v of 300 tokens 1 x 4 tiles 10.1 us, 4 x 1 8.5; a workgroup's registers leave
+// room for a second one.
+template <bool GATE, int RT, int CT, int GROUP, bool S32, bool DIRECT>
 __global__ void __launch_bounds__(64 * kSlots, 4)
-q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
+q4_slots_kernel(Q4Out out, Parts x, const float* __restrict__ direct, Q4View w0, Q4View w1, int scale_type, int T, int rows, int cols,
                 int row_groups, int tok_groups) {
   constexpr int NA = GATE ? 2 : 1, NT = NA * RT * CT;
   extern __shared__ __attribute__((aligned(16))) unsigned char dyn[];
@@ -558,6 +586,10 @@ q4_slots_kernel(Q4Out out, Parts x, Q4View w0, Q4View w1, int scale_type, int T,
     for (int n = 0; n < NA; ++n) a.w[n].load(w[n], b, g);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
+      if constexpr (DIRECT) {
+        split_tile<GROUP == kBlock>(a.hi[c], a.lo[c], a.back[c], direct, tok0 + 16 * c + r, T, cols, b, g);
+        continue;
+      }
       const size_t at = size_t(min(tok0 / 16 + c, last_tile)) * blocks + b;
       const unsigned char* parts = x.parts + at * kPartBytes;
 #pragma unroll
@@ -860,15 +892,15 @@ struct Q4Launch {
     return few_go<GATE, GROUP, S32, TP, kMost, true>(row_tiles, cus, rc) ||
            few_go<GATE, GROUP, S32, TP, kMost / 2, true>(row_tiles, cus, rc);
   }
-  template <bool GATE, int RT, int CT, int GROUP, bool S32>
+  template <bool GATE, int RT, int CT, int GROUP, bool S32, bool DIRECT>
   int slots() const {
     constexpr int kLds = kSlots * (GATE ? 2 : 1) * RT * CT * 1024;
     static_assert(kLds <= 64 * 1024, "two workgroups of a compute unit");
     const int64_t row_groups = (int64_t(rows) + 16 * RT - 1) / (16 * RT);
     const int64_t tok_groups = (int64_t(T) + 16 * CT - 1) / (16 * CT);
     if (row_groups * tok_groups * 64 * kSlots > int64_t(UINT32_MAX)) return too_many();
-    hipLaunchKernelGGL((q4_slots_kernel<GATE, RT, CT, GROUP, S32>), dim3(unsigned(row_groups * tok_groups)),
-                       dim3(64 * kSlots), kLds, stream, out, parts, w0, w1, scale_type, T, rows, cols,
+    hipLaunchKernelGGL((q4_slots_kernel<GATE, RT, CT, GROUP, S32, DIRECT>), dim3(unsigned(row_groups * tok_groups)),
+                       dim3(64 * kSlots), kLds, stream, out, parts, x, w0, w1, scale_type, T, rows, cols,
                        int(row_groups), int(tok_groups));
     return IE_HIP_OK;
   }
@@ -895,6 +927,13 @@ struct Q4Launch {
                        w0, w1, scale_type, T, rows, cols, int(row_tiles), int(tok_tiles));
     return true;
   }
+  template <bool GATE, int GROUP, bool S32, bool DIRECT>
+  int by_slots(int64_t row_tiles, int64_t tok_tiles, int64_t cus) const {
+    constexpr int kMost = GATE ? 2 : 4;  // row tiles of a workgroup: as many as leave every unit one
+    if ((row_tiles + kMost - 1) / kMost * tok_tiles >= cus) return slots<GATE, kMost, 1, GROUP, S32, DIRECT>();
+    if (!GATE && (row_tiles + 1) / 2 * tok_tiles >= cus) return slots<GATE, 2, 1, GROUP, S32, DIRECT>();
+    return slots<GATE, 1, 1, GROUP, S32, DIRECT>();
+  }
   template <bool GATE, int GROUP, bool S32>
   int run() const {
     const int64_t row_tiles = (int64_t(rows) + 15) / 16;
@@ -909,16 +948,20 @@ struct Q4Launch {
       return fail(IE_HIP_EINVAL, std::string(who) + ": activations past a workgroup's memory");
     }
     const int64_t tok_tiles = (int64_t(T) + 15) / 16, blocks = (int64_t(cols) + kBlock - 1) / kBlock;
+    // One block a slot, and a tile or less for each unit or one group of row tiles: the waves split what
+    // they multiply, a launch less (us, parts first and not: 40 tokens of 896 columns by 1,152 rows 5.8 and
+    // 5.5, 2,048 by 64 11.0 and 5.9). With more blocks a wave has nothing under way while it splits (20 of
+    // 4,864 by 128 10.4 and 14.3), with more tiles it splits the same tokens too often (64 of 896 by 1,152
+    // 6.5 and 7.6).
+    if (cols <= kSlots * kBlock && (row_tiles <= (GATE ? 2 : 4) || row_tiles * tok_tiles <= cus))
+      return by_slots<GATE, GROUP, S32, true>(row_tiles, tok_tiles, cus);
     if (tok_tiles * blocks * 256 > int64_t(UINT32_MAX)) return too_many();
     hipLaunchKernelGGL(q4_split_kernel<GROUP == kBlock>, dim3(unsigned(tok_tiles * blocks)), dim3(256), 0,
                        stream, parts, x, T, cols, int(blocks));
     if (T <= 32 ? tiles<GATE, GROUP, S32, 1>(cus, &rc)
                 : T <= 64 ? tiles<GATE, GROUP, S32, 2>(cus, &rc) : tiles<GATE, GROUP, S32, 4>(cus, &rc))
       return rc;
-    constexpr int kMost = GATE ? 2 : 4;  // row tiles of a workgroup: as many as leave every unit one
-    if ((row_tiles + kMost - 1) / kMost * tok_tiles >= cus) return slots<GATE, kMost, 1, GROUP, S32>();
-    if (!GATE && (row_tiles + 1) / 2 * tok_tiles >= cus) return slots<GATE, 2, 1, GROUP, S32>();
-    return slots<GATE, 1, 1, GROUP, S32>();
+    return by_slots<GATE, GROUP, S32, false>(row_tiles, tok_tiles, cus);
   }
   template <bool GATE, int GROUP>
   int run() const {

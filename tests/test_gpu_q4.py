@@ -119,6 +119,28 @@ def test_a_token_does_not_depend_on_its_batch(ie, dev):
         assert np.array_equal(alone, want[399:])
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("cols", [32, 992, 1024, 1056])
+def test_few_rows_of_many_tokens(ie, dev, cols, group):
+    """Matrices of up to a few row tiles, on both sides of the rules that let their products split the
+    tokens: bit for bit what the tokens are alone, each kind of product."""
+    rng = np.random.default_rng(cols + group)
+    for rows, T in ((31, 700), (64, 2041), (65, 700), (250, 250), (256, 256), (257, 257)):
+        m, _ = matrix(ie, dev, rng, rows, cols, group, zero=True)
+        up_m, _ = matrix(ie, dev, rng, rows, cols, group, zero=True)
+        x = activations(rng, T, cols)
+        x[T // 2, 0] = np.inf
+        x[T - 1] = 0
+        got = product(ie, dev, m, x).view(np.uint32)
+        out = torch.full((T, rows), float("nan"), device=dev)
+        ie.gate_up_silu_q4(out, up(dev, x), m, up_m, workspace=ie.matmul_q4_workspace(T, cols, dev))
+        for t in (0, 15, 16, T // 2, T - 1):
+            assert np.array_equal(got[t:t + 1], product(ie, dev, m, x[t:t + 1]).view(np.uint32)), (rows, T, t)
+            one = torch.empty((1, rows), device=dev)
+            ie.gate_up_silu_q4(one, up(dev, x[t:t + 1]), m, up_m)
+            assert torch.equal(one.view(torch.int32), out[t:t + 1].view(torch.int32)), (rows, T, t)
+
+
 @pytest.mark.parametrize("cols", [1952, 2080])
 @pytest.mark.parametrize("group", [32, 128])
 def test_many_tokens_on_both_sides_of_a_rule(ie, dev, cols, group):
